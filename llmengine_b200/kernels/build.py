@@ -55,6 +55,8 @@ SOURCES: Dict[str, str] = {
     "sampling": "sampling.cu",
     "gemm_skinny": "gemm_skinny.cu",
     "gemm_tcgen05": "gemm_tcgen05.cu",
+    # rows of 8-bit numbers with a scale each: of a norm, of a gate, of rows as they are
+    "rows_e4m3": "rows_e4m3.cu",
     "utility": "utility.cu",
     # the step executor (host code): walks a model's plan and launches the kernels of the other libraries
     "executor": "executor.cu",

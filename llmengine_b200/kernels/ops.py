@@ -368,6 +368,49 @@ class CudaOps:
             return c_void_p(_raw_stream(self._device_index))
         return c_void_p(torch.cuda.current_stream().cuda_stream)
 
+    # ------------------------------------------------------------------ operands of the methods that check what they are given
+    def _operand(self, what: str, name: str, t: torch.Tensor, dtypes, shape=None, dense: bool = False) -> torch.Tensor:
+        """`t` is a tensor on this device of one of the types and of the shape (None: any extent), its last dimension without
+        gaps, with `dense` none at all."""
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != self._device_index:
+            raise KernelError(f"{what}: {name} must be a tensor on cuda:{self._device_index}, got {getattr(t, 'device', type(t).__name__)}")
+        if t.dtype not in dtypes:
+            raise KernelError(f"{what}: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+        if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape))):
+            raise KernelError(f"{what}: {name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
+        if t.numel() and (not t.is_contiguous() if dense else (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise KernelError(f"{what}: {name} must {'be contiguous' if dense else 'have rows without gaps'}, got strides {tuple(t.stride())}")
+        return t
+
+    @staticmethod
+    def _row_stride(t: torch.Tensor) -> int:
+        """Elements from one row of a matrix to the next; a matrix of one row has none, so its width stands for it."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    @staticmethod
+    def _apart(what: str, out: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+        """`out` lies over none of the others' memory."""
+        def span(t):
+            return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+        if out.numel():
+            a, b = span(out)
+            for t in others:
+                if t is not None and t.numel():
+                    c, d = span(t)
+                    if a < d and c < b:
+                        raise KernelError(f"{what}: an output lies over another operand")
+
+    def _launch(self, key: str, entry: str, what: str, *args) -> None:
+        """One entry point of a library on torch's current stream, with this device the current one."""
+        lib = self._lib(key)
+        fn = getattr(lib, entry)
+        if torch.cuda.current_device() == self._device_index:
+            rc = fn(*args, self._stream())
+        else:
+            with torch.cuda.device(self._device_index):
+                rc = fn(*args, self._stream())
+        self._check(lib, rc, what)
+
     # ------------------------------------------------------------------ kernels
     def embedding(self, ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         lib = self._lib("elementwise")
@@ -540,6 +583,74 @@ class CudaOps:
                              c_int(_code(out.dtype)), c_int(out.shape[0]), c_int(out.shape[1]), self._stream())
         self._check(lib, rc, "swiglu")
         return out
+
+    # ------------------------------------------------------------------ rows of 8-bit numbers
+    def _quantised_places(self, what: str, rows: int, size: int, out: torch.Tensor, scales: torch.Tensor, *read: Optional[torch.Tensor]) -> None:
+        if rows and not size:
+            raise KernelError(f"{what}: the rows have no values")
+        self._operand(what, "out", out, (torch.float8_e4m3fn,), (rows, size))
+        self._operand(what, "scales", scales, (torch.float32,), (rows,), dense=True)
+        if rows > 1 and out.stride(0) < size:
+            raise KernelError(f"{what}: the rows of out lie over one another")
+        self._apart(what, out, scales, *read)
+        self._apart(what, scales, *read)
+
+    def rmsnorm_e4m3(self, x: torch.Tensor, gain: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
+                     delta: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None):
+        """t = x + delta (written to `total`, or back to x where there is none), h = t / sqrt(mean(t^2) + eps) * gain, and h as 8-bit
+        rows: scales[i] = max(max |h_i|, 2^-100) / 448, out[i] = h_i / scales[i] in float8_e4m3fn.  x and `total` 32-bit [T, D]; `delta`
+        and `gain` 32-bit or bfloat16.  A row that holds a NaN or an infinity gets a scale that is no finite number.  Returns (out, scales)."""
+        what, both = "rmsnorm_e4m3", (torch.float32, torch.bfloat16)
+        rows, size = self._operand(what, "x", x, (torch.float32,), (None, None), dense=True).shape
+        self._operand(what, "gain", gain, both, (size,), dense=True)
+        if not eps > 0.0:
+            raise KernelError(f"{what}: eps must be positive, got {eps}")
+        if delta is not None:
+            self._operand(what, "delta", delta, both, (rows, size), dense=True)
+            if total is None or total is x:
+                total = x
+            else:
+                self._apart(what, self._operand(what, "total", total, (torch.float32,), (rows, size), dense=True), x, gain, delta)
+            if total is x:
+                self._apart(what, x, delta, gain)
+        elif total is not None:
+            raise KernelError(f"{what}: without a delta there is no sum to write")
+        self._quantised_places(what, rows, size, out, scales, x, gain, delta, total)
+        self._operand(what, "out", out, (torch.float8_e4m3fn,), dense=True)
+        if rows:
+            self._launch("rows_e4m3", "llme_rmsnorm_e4m3", what, c_void_p(x.data_ptr()), c_void_p(_ptr(delta)),
+                         c_int(_code(delta.dtype) if delta is not None else 0), c_void_p(gain.data_ptr()), c_int(_code(gain.dtype)),
+                         c_void_p(_ptr(total)), c_void_p(out.data_ptr()), c_void_p(scales.data_ptr()), c_int(rows), c_int(size), c_float(eps))
+        return out, scales
+
+    def rows_e4m3(self, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
+        """The rows of x [T, D] (32-bit or bfloat16, any row stride) as 8-bit rows: scales[i] = max(max |x_i|, 2^-100) / 448,
+        out[i] = x_i / scales[i] in float8_e4m3fn (any row stride).  Returns (out, scales)."""
+        what = "rows_e4m3"
+        rows, size = self._operand(what, "x", x, (torch.float32, torch.bfloat16), (None, None)).shape
+        if rows > 1 and x.stride(0) < size:
+            raise KernelError(f"{what}: the rows of x lie over one another")
+        self._quantised_places(what, rows, size, out, scales, x)
+        if rows:
+            self._launch("rows_e4m3", "llme_rows_e4m3", what, c_void_p(x.data_ptr()), c_int(_code(x.dtype)), c_longlong(self._row_stride(x)),
+                         c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)), c_void_p(scales.data_ptr()), c_int(rows), c_int(size))
+        return out, scales
+
+    def swiglu_e4m3(self, gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
+        """silu(gate) * up of gate_up [T, 2 D] = [gate | up] (32-bit or bfloat16, any row stride) as 8-bit rows, as `rows_e4m3` makes
+        them.  Returns (out, scales)."""
+        what = "swiglu_e4m3"
+        rows, both = self._operand(what, "gate_up", gate_up, (torch.float32, torch.bfloat16), (None, None)).shape
+        if both % 2:
+            raise KernelError(f"{what}: gate_up must have an even number of columns, got {both}")
+        if rows > 1 and gate_up.stride(0) < both:
+            raise KernelError(f"{what}: the rows of gate_up lie over one another")
+        self._quantised_places(what, rows, both // 2, out, scales, gate_up)
+        if rows:
+            self._launch("rows_e4m3", "llme_swiglu_e4m3", what, c_void_p(gate_up.data_ptr()), c_int(_code(gate_up.dtype)),
+                         c_longlong(self._row_stride(gate_up)), c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)),
+                         c_void_p(scales.data_ptr()), c_int(rows), c_int(both // 2))
+        return out, scales
 
     def _run_one(self, record) -> None:
         """One operation through the executor, for all rows of its input (what `linear` and `linear_swiglu` below do):
