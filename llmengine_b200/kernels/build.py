@@ -57,6 +57,9 @@ SOURCES: Dict[str, str] = {
     "gemm_tcgen05": "gemm_tcgen05.cu",
     # rows of 8-bit numbers with a scale each: of a norm, of a gate, of rows as they are
     "rows_e4m3": "rows_e4m3.cu",
+    # products with weights of 8 bits (and rows of 8 bits) and of 4 bits
+    "gemm_e4m3": "gemm_e4m3.cu",
+    "gemm_int4": "gemm_int4.cu",
     "utility": "utility.cu",
     # the step executor (host code): walks a model's plan and launches the kernels of the other libraries
     "executor": "executor.cu",

@@ -652,6 +652,59 @@ class CudaOps:
                          c_void_p(scales.data_ptr()), c_int(rows), c_int(both // 2))
         return out, scales
 
+    # ------------------------------------------------------------------ products with weights of 8 and 4 bits
+    def _product_places(self, what: str, x: torch.Tensor, n: int, out: torch.Tensor, dtypes, *read: Optional[torch.Tensor]) -> None:
+        rows = x.shape[0]
+        self._operand(what, "out", out, dtypes, (rows, n))
+        for name, t in (("x", x), ("out", out)):
+            if rows > 1 and t.stride(0) < t.shape[1]:
+                raise KernelError(f"{what}: the rows of {name} lie over one another")
+        self._apart(what, out, x, *read)
+
+    def linear_e4m3(self, x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        """out[m, n] = x_scales[m] w_scales[n] (x[m] . w[n]) for x [M, K] and w [N, K] in float8_e4m3fn, scales 32-bit, out [M, N] 32-bit
+        or bfloat16; sums are 32-bit.  K is a multiple of 16, the rows of x and w begin on 16 bytes (any such row stride)."""
+        what, f8 = "linear_e4m3", (torch.float8_e4m3fn,)
+        M, K = self._operand(what, "x", x, f8, (None, None)).shape
+        N = self._operand(what, "w", w, f8, (None, K)).shape[0]
+        self._operand(what, "x_scales", x_scales, (torch.float32,), (M,), dense=True)
+        self._operand(what, "w_scales", w_scales, (torch.float32,), (N,), dense=True)
+        self._product_places(what, x, N, out, (torch.float32, torch.bfloat16), w, x_scales, w_scales)
+        if M and N:
+            self._launch("gemm_e4m3", "llme_gemm_e4m3", what, c_void_p(x.data_ptr()), c_longlong(self._row_stride(x)), c_void_p(x_scales.data_ptr()),
+                         c_void_p(w.data_ptr()), c_longlong(self._row_stride(w)), c_void_p(w_scales.data_ptr()), c_void_p(out.data_ptr()),
+                         c_int(_code(out.dtype)), c_longlong(self._row_stride(out)), c_int(M), c_int(N), c_int(K))
+        return out
+
+    @staticmethod
+    def int4_group(k: int, groups: int) -> int:
+        """How many of k values share a scale when a row has `groups` scales: 32, 64 or 128 (where one scale serves the whole row, the
+        least that covers it)."""
+        for group in (32, 64, 128):
+            if -(-k // group) == groups:
+                return group
+        raise KernelError(f"linear_int4: {groups} scales a row fit no group of 32, 64 or 128 of {k} values")
+
+    def linear_int4(self, x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, out: torch.Tensor,
+                    zeros: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """out[m, n] = sum over k of x[m, k] scales[n, g] (c[n, k] - zeros[n, g]), g = k // group: x [M, K] and out [M, N] bfloat16; `w`
+        uint8 [N, ceil(K / 128) * 64], the codes c as weights.quantize.pack_int4 lays them; scales [N, ceil(K / group)] bfloat16 for a
+        group of 32, 64 or 128; zeros uint8 of that shape with values 0..15 (None: 8 everywhere).  Sums are 32-bit.  K is a multiple
+        of 8, the rows of x and w begin on 16 bytes (any such row stride)."""
+        what = "linear_int4"
+        M, K = self._operand(what, "x", x, (torch.bfloat16,), (None, None)).shape
+        N = self._operand(what, "w", w, (torch.uint8,), (None, -(-K // 128) * 64)).shape[0]
+        groups = self._operand(what, "scales", scales, (torch.bfloat16,), (N, None), dense=True).shape[1]
+        if zeros is not None:
+            self._operand(what, "zeros", zeros, (torch.uint8,), (N, groups), dense=True)
+        group = self.int4_group(K, groups)
+        self._product_places(what, x, N, out, (torch.bfloat16,), w, scales, zeros)
+        if M and N:
+            self._launch("gemm_int4", "llme_gemm_int4", what, c_void_p(x.data_ptr()), c_longlong(self._row_stride(x)), c_void_p(w.data_ptr()),
+                         c_longlong(self._row_stride(w)), c_void_p(scales.data_ptr()), c_void_p(_ptr(zeros)), c_longlong(groups), c_int(group),
+                         c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)), c_int(M), c_int(N), c_int(K))
+        return out
+
     def _run_one(self, record) -> None:
         """One operation through the executor, for all rows of its input (what `linear` and `linear_swiglu` below do):
         the executor's choice of kernel, outside any model."""

@@ -1,0 +1,69 @@
+"""How matrices are rounded to 8 and 4 bits, and how 4-bit codes lie."""
+import pytest
+import torch
+
+from llmengine_b200.weights import quantize as qz
+
+
+def _w(n, k, seed=0):
+    return torch.randn(n, k, generator=torch.Generator().manual_seed(seed)) * 0.05
+
+
+@pytest.mark.parametrize("k", [1, 8, 31, 32, 127, 128, 129, 200, 384])
+def test_codes_come_back(k):
+    codes = torch.randint(0, 16, (5, k), generator=torch.Generator().manual_seed(k)).to(torch.uint8)
+    packed = qz.pack_int4(codes)
+    assert packed.shape == (5, -(-k // 128) * 64) and packed.dtype == torch.uint8
+    assert torch.equal(qz.unpack_int4(packed, k), codes)
+
+
+def test_where_a_code_lies():
+    """Value 32 j + 8 q + e of a block is in word 4 q + j, at bits 4 (e / 2) + 16 (e % 2)."""
+    for k in range(256):
+        codes = torch.zeros(1, 256, dtype=torch.uint8)
+        codes[0, k] = 11
+        words = qz.pack_int4(codes).view(torch.int32).tolist()[0]
+        block, j, q, e = k // 128, k % 128 // 32, k % 32 // 8, k % 8
+        want = [0] * 32
+        want[16 * block + 4 * q + j] = 11 << (4 * (e // 2) + 16 * (e % 2))
+        assert [w & 0xFFFFFFFF for w in words] == want
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("k", [8, 100, 512])
+def test_4_bits_are_near(group, zeros, k):
+    w = _w(9, k, seed=group + k)
+    packed, scales, zero = qz.quantize_int4(w, group, zeros)
+    assert scales.shape == (9, -(-k // group)) and scales.dtype == torch.bfloat16 and (zero is None) != zeros
+    back = qz.dequantize_int4(packed, scales, zero, k, group)
+    at = torch.arange(k) // group
+    # half a step of the scale; the scale itself is rounded to bfloat16 (2^-8), which can move the ends of the range, 7 or 15 steps away,
+    # and a zero point rounded by half a step cuts off as much at one end
+    step = scales.float()[:, at]
+    assert torch.all((back - w).abs() <= step * (0.5 + (0.5 if zeros else 0.0) + 15 * 2.0 ** -8) + 1e-12)
+
+
+def test_8_bits_are_near():
+    w = _w(7, 300)
+    w[3] = 0
+    q, scales = qz.quantize_e4m3(w)
+    assert q.dtype == torch.float8_e4m3fn and scales.shape == (7,) and torch.all(q[3].float() == 0) and torch.all(scales > 0)
+    y = w / scales[:, None]
+    assert torch.all((q.float() - y).abs() <= torch.maximum(y.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10)) * (1 + 2.0 ** -20))
+    assert torch.all(q.float().abs().amax(1)[[0, 1, 2, 4, 5, 6]] == 448)
+
+
+def test_rows_of_zeros_in_4_bits():
+    for zeros in (False, True):
+        packed, scales, zero = qz.quantize_int4(torch.zeros(3, 64), 32, zeros)
+        assert torch.all(qz.dequantize_int4(packed, scales, zero, 64, 32) == 0) and torch.all(scales.float() > 0)
+
+
+def test_refusals():
+    for call in (lambda: qz.quantize_int4(_w(4, 64), 48), lambda: qz.quantize_int4(torch.full((2, 64), float("nan")), 64),
+                 lambda: qz.quantize_e4m3(torch.full((2, 64), float("inf"))), lambda: qz.quantize_e4m3(torch.ones(2, 3, 4)),
+                 lambda: qz.pack_int4(torch.full((2, 64), 16)), lambda: qz.pack_int4(torch.full((2, 64), -1)),
+                 lambda: qz.pack_int4(torch.zeros(2, 64)), lambda: qz.unpack_int4(torch.zeros(2, 64, dtype=torch.uint8), 129)):
+        with pytest.raises(ValueError):
+            call()
