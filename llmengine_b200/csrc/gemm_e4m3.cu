@@ -9,6 +9,7 @@
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
 #include "common.cuh"
+#include "operands.cuh"
 
 LLME_API const char* llme_last_error() { return llme_error_buffer(); }
 
@@ -114,6 +115,8 @@ LLME_API int llme_gemm_e4m3(const void* x, long long ldx, const float* xs, const
     if (K <= 0 || K % 16 || ldx % 16 || ldw % 16 || ldx < K || ldw < K) LLME_REFUSE("gemm_e4m3: K=%d ldx=%lld ldw=%lld is not supported (multiples of 16, rows that do not overlap)", K, ldx, ldw);
     if (((uintptr_t)x | (uintptr_t)w) % 16) LLME_REFUSE("gemm_e4m3: operands must be 16-byte aligned");
     if (ldo < N) LLME_REFUSE("gemm_e4m3: output row stride shorter than the row");
+    if (meets(span(out, M, N, ldo, out_dtype == LLME_F32 ? 4 : 2), {span(x, M, K, ldx, 1), span(w, N, K, ldw, 1), span(xs, 1, M, M, 4), span(ws, 1, N, N, 4)}))
+        LLME_REFUSE("gemm_e4m3: the output lies over an operand");
     if ((M + 15) / 16 > 65535) LLME_REFUSE("gemm_e4m3: %d rows are too many for one launch", M);
     const Args a{(const unsigned char*)x, ldx, xs, (const unsigned char*)w, ldw, ws, out, ldo, M, N, K};
     if (out_dtype == LLME_F32) return launch<float>(a, stream);

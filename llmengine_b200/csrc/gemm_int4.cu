@@ -13,6 +13,7 @@
 //
 // The reference's weight-only product has 8-bit blocks (src/runtime/kernels/cuda_kernels.cu:296-358); it has none of 4 bits.
 #include "common.cuh"
+#include "operands.cuh"
 
 LLME_API const char* llme_last_error() { return llme_error_buffer(); }
 
@@ -154,6 +155,9 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     if (lds < (K + group - 1LL) / group) LLME_REFUSE("gemm_int4: rows of %lld scales are too short", lds);
     if (((uintptr_t)x | (uintptr_t)w) % 16) LLME_REFUSE("gemm_int4: operands must be 16-byte aligned");
     if (ldo < N) LLME_REFUSE("gemm_int4: output row stride shorter than the row");
+    const long long groups = (K + group - 1LL) / group;
+    if (meets(span(out, M, N, ldo, 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
+        LLME_REFUSE("gemm_int4: the output lies over an operand");
     if ((M + 15) / 16 > 65535) LLME_REFUSE("gemm_int4: %d rows are too many for one launch", M);
     const Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K};
     if (group == 32) return launch<1>(a, stream);

@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "operands.cuh"
 
 LLME_API const char* llme_last_error() { return llme_error_buffer(); }
 
@@ -29,32 +30,32 @@ typedef __nv_bfloat16 bf16;
 constexpr float LARGEST = 448.0f;
 constexpr float LEAST = 7.8886090522101181e-31f;        // 2^-100
 
-// N values (8, 2 or 1) of a row as 32-bit ones
-template <int N> __device__ __forceinline__ void load(const float* p, float (&v)[N]) {
-    if constexpr (N == 8) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else if constexpr (N == 2) {
-        const float2 a = *reinterpret_cast<const float2*>(p);
-        v[0] = a.x; v[1] = a.y;
-    } else {
-        v[0] = p[0];
-    }
-}
-template <int N> __device__ __forceinline__ void load(const bf16* p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = __bfloat162float(p[0]);
-    } else {
-        unsigned raw[N / 2];
-        if constexpr (N == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
-        else raw[0] = *reinterpret_cast<const unsigned*>(p);
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            v[2 * i] = __uint_as_float(raw[i] << 16);
-            v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+// N values (8, 2 or 1) of a row as they lie in memory: they stay so until they are needed, bfloat16 ones in half the registers.
+template <typename T, int N> struct Piece;
+template <int N> struct Piece<float, N> {
+    float v[N];
+    __device__ __forceinline__ void load(const float* p) {
+        if constexpr (N == 8) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else if constexpr (N == 2) {
+            const float2 a = *reinterpret_cast<const float2*>(p);
+            v[0] = a.x; v[1] = a.y;
+        } else {
+            v[0] = p[0];
         }
     }
-}
+    __device__ __forceinline__ float at(int i) const { return v[i]; }
+};
+template <int N> struct Piece<bf16, N> {
+    unsigned raw[(N + 1) / 2];
+    __device__ __forceinline__ void load(const bf16* p) {
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
+        else if constexpr (N == 2) raw[0] = *reinterpret_cast<const unsigned*>(p);
+        else raw[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16); }
+};
 template <int N> __device__ __forceinline__ void store(float* p, const float (&v)[N]) {
     if constexpr (N == 8) {
         reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -84,38 +85,55 @@ template <int N> __device__ __forceinline__ void store_e4m3(unsigned char* p, co
     }
 }
 
-// ---- where a row comes from.  fetch() brings N values at column j, and what else the column needs into `extra`; finish() makes the
-// values that are quantised of them.
+// ---- where a row comes from.  fetch() brings what N values at column j are made of, values() makes them.
 template <typename T> struct FromRows {
-    static constexpr bool NORM = false;
+    static constexpr bool NORM = false, EXACT = true;
+    static constexpr int MOST = 4;                 // pieces of eight values a thread holds where rows are many
     const T* x; long long ldx;
-    template <int N> __device__ __forceinline__ void fetch(int row, int j, float (&v)[N], float (&)[N]) const { load<N>(x + row * ldx + j, v); }
-    template <int N> __device__ __forceinline__ void finish(int, int, float (&)[N], float (&)[N]) const {}
+    template <int N> using Raw = Piece<T, N>;
+    template <int N> __device__ __forceinline__ void fetch(int row, int j, Raw<N>& r) const { r.load(x + row * ldx + j); }
+    template <int N> __device__ __forceinline__ void values(int, int, const Raw<N>& r, float (&v)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = r.at(i);
+    }
 };
 template <typename T> struct FromGate {
-    static constexpr bool NORM = false;
+    static constexpr bool NORM = false, EXACT = false;
+    static constexpr int MOST = 6;
     const T* x; long long ldx; int inter;
-    template <int N> __device__ __forceinline__ void fetch(int row, int j, float (&v)[N], float (&up)[N]) const {
-        load<N>(x + row * ldx + j, v);
-        load<N>(x + row * ldx + inter + j, up);
+    template <int N> struct Raw { Piece<T, N> gate, up; };
+    template <int N> __device__ __forceinline__ void fetch(int row, int j, Raw<N>& r) const {
+        r.gate.load(x + row * ldx + j);
+        r.up.load(x + row * ldx + inter + j);
     }
-    template <int N> __device__ __forceinline__ void finish(int, int, float (&v)[N], float (&up)[N]) const {
+    template <int N> __device__ __forceinline__ void values(int, int, const Raw<N>& r, float (&v)[N]) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = sizeof(T) == 2 ? silu_mul_bf16(v[i], up[i]) : v[i] / (1.0f + expf(-v[i])) * up[i];
+        for (int i = 0; i < N; ++i) {
+            const float g = r.gate.at(i);
+            v[i] = sizeof(T) == 2 ? silu_mul_bf16(g, r.up.at(i)) : g / (1.0f + expf(-g)) * r.up.at(i);
+        }
     }
 };
 // D: type of the contribution, or void where none is pending
 template <typename D, typename G> struct FromNorm {
-    static constexpr bool NORM = true;
+    static constexpr bool NORM = true, EXACT = false;
+    static constexpr int MOST = 1;                 // (a row's squares are added in an order that must not depend on how many rows there are)
     const float* x; const D* delta; const G* gain; float* total; int size; float eps;
-    template <int N> __device__ __forceinline__ void fetch(int row, int j, float (&v)[N], float (&d)[N]) const {
-        load<N>(x + (long long)row * size + j, v);
-        if constexpr (!std::is_void_v<D>) load<N>(delta + (long long)row * size + j, d);
+    template <int N> using Gain = Piece<G, N>;
+    template <int N> struct Raw {
+        Piece<float, N> x;
+        Piece<std::conditional_t<std::is_void_v<D>, bf16, D>, N> d;
+    };
+    template <int N> __device__ __forceinline__ void fetch(int row, int j, Raw<N>& r) const {
+        r.x.load(x + (long long)row * size + j);
+        if constexpr (!std::is_void_v<D>) r.d.load(delta + (long long)row * size + j);
     }
-    template <int N> __device__ __forceinline__ void finish(int row, int j, float (&v)[N], float (&d)[N]) const {
+    template <int N> __device__ __forceinline__ void values(int row, int j, const Raw<N>& r, float (&v)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = r.x.at(i);
         if constexpr (!std::is_void_v<D>) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += d[i];
+            for (int i = 0; i < N; ++i) v[i] += r.d.at(i);
             store<N>(total + (long long)row * size + j, v);
         }
     }
@@ -123,6 +141,13 @@ template <typename D, typename G> struct FromNorm {
 
 // The largest of several |v| as bits: for numbers without a sign they are in the order of the values, infinity above all, NaN above that.
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// v / a from 1 / a and one correction: the quotient's error is known exactly, v - q a.  (Values of a few bits over a scale of theirs meet the
+// middle between two e4m3 numbers often, and v times 1 / a would fall to either side of it.)
+__device__ __forceinline__ float quotient(float v, float a, float f) {
+    const float q = v * f;
+    return fmaf(fmaf(-q, a, v), f, q);
+}
 
 // A row's scale and the factor that takes its values to e4m3: `top` the largest |h| before it is multiplied by r.
 __device__ __forceinline__ float row_scale(unsigned top, float r) {
@@ -153,39 +178,59 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
     if (!BLOCK && row >= rows) return;
     const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & 31), step = BLOCK ? (int)blockDim.x : 32;
     pdl_wait();
-    float v[V][N], extra[V][N], gain[V][N];
+    typename Src::template Raw<N> raw[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int j = (t + k * step) * N;
-        if (j >= size) continue;
-        src.template fetch<N>(row, j, v[k], extra[k]);
-        if constexpr (Src::NORM) load<N>(src.gain + j, gain[k]);
-    }
-    float ss = 0.0f;
+    for (int k = 0; k < V; ++k)
+        if ((t + k * step) * N < size) src.template fetch<N>(row, (t + k * step) * N, raw[k]);
+    float v[V][N], ss = 0.0f;
     unsigned top = 0;
+    if constexpr (Src::NORM) {
+        typename Src::template Gain<N> gain[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int j = (t + k * step) * N;
-        if (j >= size) continue;
-        src.template finish<N>(row, j, v[k], extra[k]);
+        for (int k = 0; k < V; ++k)
+            if ((t + k * step) * N < size) gain[k].load(src.gain + (t + k * step) * N);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if constexpr (Src::NORM) ss = fmaf(v[k][i], v[k][i], ss);
-            top = max(top, magnitude(Src::NORM ? v[k][i] * gain[k][i] : v[k][i]));
+        for (int k = 0; k < V; ++k) {
+            const int j = (t + k * step) * N;
+            if (j >= size) continue;
+            src.template values<N>(row, j, raw[k], v[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                ss = fmaf(v[k][i], v[k][i], ss);
+                top = max(top, magnitude(v[k][i] * gain[k].at(i)));
+            }
         }
-    }
-    meet<BLOCK>(ss, top, sums, tops);
-    float r = 1.0f;
-    if constexpr (Src::NORM) r = 1.0f / sqrtf(ss / (float)size + src.eps);
-    const float a = row_scale(top, r), f = r / a;
-    if (t == 0) scales[row] = a;
+        meet<BLOCK>(ss, top, sums, tops);
+        const float r = 1.0f / sqrtf(ss / (float)size + src.eps), a = row_scale(top, r), f = r / a;
+        if (t == 0) scales[row] = a;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int j = (t + k * step) * N;
-        if (j >= size) continue;
+        for (int k = 0; k < V; ++k) {
+            const int j = (t + k * step) * N;
+            if (j >= size) continue;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[k][i] = Src::NORM ? (v[k][i] * f) * gain[k][i] : v[k][i] * f;
-        store_e4m3<N>(q + row * ldq + j, v[k]);
+            for (int i = 0; i < N; ++i) v[k][i] = (v[k][i] * f) * gain[k].at(i);
+            store_e4m3<N>(q + row * ldq + j, v[k]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int j = (t + k * step) * N;
+            if (j >= size) continue;
+            src.template values<N>(row, j, raw[k], v[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) top = max(top, magnitude(v[k][i]));
+        }
+        meet<BLOCK>(ss, top, sums, tops);
+        const float a = row_scale(top, 1.0f), f = 1.0f / a;
+        if (t == 0) scales[row] = a;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int j = (t + k * step) * N;
+            if (j >= size) continue;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[k][i] = Src::EXACT ? quotient(v[k][i], a, f) : v[k][i] * f;
+            store_e4m3<N>(q + row * ldq + j, v[k]);
+        }
     }
 }
 
@@ -198,15 +243,15 @@ __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsig
     pdl_launch_dependents();
     pdl_wait();
     const int row = (int)blockIdx.x;
-    float ss = 0.0f, v[1], extra[1], g[1];
+    typename Src::template Raw<1> raw;
+    float ss = 0.0f, v[1];
     unsigned top = 0;
     for (int j = (int)threadIdx.x; j < size; j += (int)blockDim.x) {
-        src.template fetch<1>(row, j, v, extra);
-        src.template finish<1>(row, j, v, extra);
+        src.template fetch<1>(row, j, raw);
+        src.template values<1>(row, j, raw, v);
         if constexpr (Src::NORM) {
-            load<1>(src.gain + j, g);
             ss = fmaf(v[0], v[0], ss);
-            v[0] *= g[0];
+            v[0] *= to_f32(src.gain[j]);
         }
         top = max(top, magnitude(v[0]));
     }
@@ -217,13 +262,11 @@ __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsig
     if (threadIdx.x == 0) scales[row] = a;
     for (int j = (int)threadIdx.x; j < size; j += (int)blockDim.x) {
         if constexpr (Src::NORM) {
-            load<1>((src.delta ? src.total : src.x) + (long long)row * size + j, v);
-            load<1>(src.gain + j, g);
-            v[0] = (v[0] * f) * g[0];
+            v[0] = ((src.delta ? src.total : src.x)[(long long)row * size + j] * f) * to_f32(src.gain[j]);
         } else {
-            src.template fetch<1>(row, j, v, extra);
-            src.template finish<1>(row, j, v, extra);
-            v[0] *= f;
+            src.template fetch<1>(row, j, raw);
+            src.template values<1>(row, j, raw, v);
+            v[0] = Src::EXACT ? quotient(v[0], a, f) : v[0] * f;
         }
         store_e4m3<1>(q + row * ldq + j, v);
     }
@@ -235,13 +278,31 @@ void launch_block(const Src& src, unsigned char* q, long long ldq, float* scales
     llme_launch(quantise_kernel<Src, N, V, true>, dim3(rows), dim3(threads), 0, s, src, q, ldq, scales, rows, size);
 }
 
-// `vec`: the largest of 8, 2 and 1 values whose pieces begin on their own size in every operand
+int sm_count() {
+    static const int n = [] {
+        int dev = 0, v = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+        return v;
+    }();
+    return n;
+}
+
+// `vec`: the widest pieces that every operand takes.
+// Few rows: as many threads a row as it has pieces of eight values, for the shortest way through.  Rows for several rounds of the SMs: several
+// pieces a thread, so that more rows are on an SM at once and one's loads run while another's threads meet (4,096 rows of 4,096 bfloat16
+// values, 1 / 2 / 4 / 6 pieces a thread: 13.9 / 11.7 / 10.6 / 10.9 us; the gate, 2,048 x 17,408: 62.5 with 4, 39.2 with 6, which leaves room for two
+// blocks an SM; the norm, 2,048 x 4,096 with a 32-bit contribution, gains nothing: 18.0 / 17.9 / 19.3 / 25.3), but no fewer than 128 threads (2,048
+// rows of 1,024: 3.4 us with 1, 3.7 with 2).
 template <class Src>
 int launch(const Src& src, unsigned char* q, long long ldq, float* scales, int rows, int size, int vec, cudaStream_t s) {
     const int pieces = size / vec;
+    int v = rows >= 2 * sm_count() ? (pieces / 128 < Src::MOST ? pieces / 128 : Src::MOST) : 1;
+    while (v > 1 ? pieces > v * 640 : pieces > 1024) ++v;
     if (vec == 8 && pieces <= 32) llme_launch(quantise_kernel<Src, 8, 1, false>, dim3((rows + 3) / 4), dim3(128), 0, s, src, q, ldq, scales, rows, size);
-    else if (vec == 8 && pieces <= 1024) launch_block<Src, 8, 1>(src, q, ldq, scales, rows, size, s);
-    else if (vec == 8 && pieces <= 4 * 640) launch_block<Src, 8, 4>(src, q, ldq, scales, rows, size, s);
+    else if (vec == 8 && v <= 1) launch_block<Src, 8, 1>(src, q, ldq, scales, rows, size, s);
+    else if (vec == 8 && v <= 2) launch_block<Src, 8, 2>(src, q, ldq, scales, rows, size, s);
+    else if (vec == 8 && v <= 4) launch_block<Src, 8, 4>(src, q, ldq, scales, rows, size, s);
+    else if (vec == 8 && v <= 6) launch_block<Src, 8, 6>(src, q, ldq, scales, rows, size, s);
     else if (vec >= 2 && size / 2 <= 8 * 640) launch_block<Src, 2, 8>(src, q, ldq, scales, rows, size, s);
     else llme_launch(quantise_long_kernel<Src>, dim3(rows), dim3(size >= 2048 ? 512 : 128), 0, s, src, q, ldq, scales, rows, size);
     LLME_LAUNCH_STATUS();
@@ -278,6 +339,11 @@ LLME_API int llme_rmsnorm_e4m3(const float* x, const void* delta, int delta_dtyp
     if (!x || !gain || !q || !scales || size <= 0) LLME_REFUSE("rmsnorm_e4m3: null pointer or non-positive size");
     if (delta && !total) LLME_REFUSE("rmsnorm_e4m3: a contribution needs a place for the sum");
     if (!(eps > 0.0f)) LLME_REFUSE("rmsnorm_e4m3: eps must be positive");
+    const Span at_x = span(x, rows, size, size, 4), at_delta = span(delta, rows, size, size, bytes_of(delta_dtype)), at_gain = span(gain, 1, size, size, bytes_of(gain_dtype));
+    const Span at_total = span(delta ? total : nullptr, rows, size, size, 4), at_q = span(q, rows, size, size, 1), at_scales = span(scales, 1, rows, rows, 4);
+    if (meets(at_q, {at_x, at_delta, at_gain, at_total, at_scales}) || meets(at_scales, {at_x, at_delta, at_gain, at_total}) ||
+        meets(at_total, {at_delta, at_gain}) || (total != x && meets(at_total, {at_x})))
+        LLME_REFUSE("rmsnorm_e4m3: an output lies over another operand");
     const int vec = pieces_of(size, {{x, size, 4}, {delta, size, bytes_of(delta_dtype)}, {gain, size, bytes_of(gain_dtype)}, {total, size, 4}, {q, size, 1}});
     unsigned char* out = (unsigned char*)q;
     if (!delta) return norm<void>(x, nullptr, gain, gain_dtype, nullptr, out, scales, rows, size, eps, vec, stream);
@@ -291,6 +357,8 @@ LLME_API int llme_rows_e4m3(const void* x, int dtype, long long ldx, void* q, lo
     if (rows <= 0) return 0;
     if (!x || !q || !scales || size <= 0) LLME_REFUSE("rows_e4m3: null pointer or non-positive size");
     if (ldx < size || ldq < size) LLME_REFUSE("rows_e4m3: a row stride is shorter than the row");
+    const Span at_x = span(x, rows, size, ldx, bytes_of(dtype)), at_q = span(q, rows, size, ldq, 1), at_scales = span(scales, 1, rows, rows, 4);
+    if (meets(at_q, {at_x, at_scales}) || meets(at_scales, {at_x})) LLME_REFUSE("rows_e4m3: an output lies over another operand");
     const int vec = pieces_of(size, {{x, ldx, bytes_of(dtype)}, {q, ldq, 1}});
     if (dtype == LLME_F32) return launch(FromRows<float>{(const float*)x, ldx}, (unsigned char*)q, ldq, scales, rows, size, vec, stream);
     if (dtype == LLME_BF16) return launch(FromRows<bf16>{(const bf16*)x, ldx}, (unsigned char*)q, ldq, scales, rows, size, vec, stream);
@@ -302,6 +370,8 @@ LLME_API int llme_swiglu_e4m3(const void* x, int dtype, long long ldx, void* q, 
     if (rows <= 0) return 0;
     if (!x || !q || !scales || size <= 0) LLME_REFUSE("swiglu_e4m3: null pointer or non-positive size");
     if (ldx < 2LL * size || ldq < size) LLME_REFUSE("swiglu_e4m3: a row stride is shorter than the row");
+    const Span at_x = span(x, rows, 2LL * size, ldx, bytes_of(dtype)), at_q = span(q, rows, size, ldq, 1), at_scales = span(scales, 1, rows, rows, 4);
+    if (meets(at_q, {at_x, at_scales}) || meets(at_scales, {at_x})) LLME_REFUSE("swiglu_e4m3: an output lies over another operand");
     const int vec = pieces_of(size, {{x, ldx, bytes_of(dtype)}, {q, ldq, 1}});
     if (dtype == LLME_F32) return launch(FromGate<float>{(const float*)x, ldx, size}, (unsigned char*)q, ldq, scales, rows, size, vec, stream);
     if (dtype == LLME_BF16) return launch(FromGate<bf16>{(const bf16*)x, ldx, size}, (unsigned char*)q, ldq, scales, rows, size, vec, stream);

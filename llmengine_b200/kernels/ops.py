@@ -18,7 +18,7 @@ from __future__ import annotations
 import ctypes
 import os
 from ctypes import POINTER, Structure, byref, c_char_p, c_float, c_int, c_longlong, c_void_p
-from typing import Dict, Optional
+from typing import Any, Dict, Optional
 
 import torch
 
@@ -35,6 +35,7 @@ class KernelError(RuntimeError):
 
 
 _F32, _BF16 = 0, 1
+_FLOAT, _FLOATS, _BF16S, _E4M3, _BYTES = (torch.float32,), (torch.float32, torch.bfloat16), (torch.bfloat16,), (torch.float8_e4m3fn,), (torch.uint8,)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -116,6 +117,7 @@ class CudaOps:
             raise KernelsUnavailable(f"device {device} is not a CUDA device")
         self._device_index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self._libs: Dict[str, ctypes.CDLL] = {}
+        self._typed: Dict[str, Any] = {}       # entry points whose argument types are set
         self._sms = None
         self._direct = 0           # kernels launched through the methods below (the executor counts its own)
         self._xlib = self._lib("executor")
@@ -369,47 +371,45 @@ class CudaOps:
         return c_void_p(torch.cuda.current_stream().cuda_stream)
 
     # ------------------------------------------------------------------ operands of the methods that check what they are given
+    # (Each check asks the usual case first: a call of a few microseconds on the GPU should not take many times that here.)
     def _operand(self, what: str, name: str, t: torch.Tensor, dtypes, shape=None, dense: bool = False) -> torch.Tensor:
-        """`t` is a tensor on this device of one of the types and of the shape (None: any extent), its last dimension without
-        gaps, with `dense` none at all."""
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != self._device_index:
+        """`t` is a tensor on this device of one of the types and of the shape (None: any matrix), its last dimension without gaps,
+        with `dense` none at all."""
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._device_index:
             raise KernelError(f"{what}: {name} must be a tensor on cuda:{self._device_index}, got {getattr(t, 'device', type(t).__name__)}")
         if t.dtype not in dtypes:
             raise KernelError(f"{what}: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-        if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape))):
-            raise KernelError(f"{what}: {name} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(t.shape)}")
-        if t.numel() and (not t.is_contiguous() if dense else (t.shape[-1] > 1 and t.stride(-1) != 1)):
+        if t.shape != shape if shape is not None else t.dim() != 2:
+            raise KernelError(f"{what}: {name} must {'be a matrix' if shape is None else f'have shape {tuple(shape)}'}, got shape {tuple(t.shape)}")
+        if not t.is_contiguous() and (dense or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1)):
             raise KernelError(f"{what}: {name} must {'be contiguous' if dense else 'have rows without gaps'}, got strides {tuple(t.stride())}")
         return t
 
     @staticmethod
     def _row_stride(t: torch.Tensor) -> int:
         """Elements from one row of a matrix to the next; a matrix of one row has none, so its width stands for it."""
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        rows, cols = t.shape
+        return t.stride(0) if rows > 1 else cols
 
-    @staticmethod
-    def _apart(what: str, out: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-        """`out` lies over none of the others' memory."""
-        def span(t):
-            return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-        if out.numel():
-            a, b = span(out)
-            for t in others:
-                if t is not None and t.numel():
-                    c, d = span(t)
-                    if a < d and c < b:
-                        raise KernelError(f"{what}: an output lies over another operand")
+    def _entry(self, key: str, entry: str, *types):
+        """A library's entry point with its argument types; the last argument is the stream."""
+        fn = self._typed.get(entry)
+        if fn is None:
+            fn = getattr(self._lib(key), entry)
+            fn.argtypes = [*types, c_void_p]
+            self._typed[entry] = fn
+        return fn
 
-    def _launch(self, key: str, entry: str, what: str, *args) -> None:
-        """One entry point of a library on torch's current stream, with this device the current one."""
-        lib = self._lib(key)
-        fn = getattr(lib, entry)
+    def _launch(self, key: str, what: str, fn, *args) -> None:
+        """An entry point on torch's current stream of this device, with this device the current one."""
         if torch.cuda.current_device() == self._device_index:
             rc = fn(*args, self._stream())
         else:
             with torch.cuda.device(self._device_index):
                 rc = fn(*args, self._stream())
-        self._check(lib, rc, what)
+        if rc != 0:
+            raise KernelError(f"{what}: {self._libs[key].llme_last_error().decode('utf-8', 'replace')} (code {rc})")
+        self._direct += 1
 
     # ------------------------------------------------------------------ kernels
     def embedding(self, ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -585,95 +585,85 @@ class CudaOps:
         return out
 
     # ------------------------------------------------------------------ rows of 8-bit numbers
-    def _quantised_places(self, what: str, rows: int, size: int, out: torch.Tensor, scales: torch.Tensor, *read: Optional[torch.Tensor]) -> None:
+    def _quantised_places(self, what: str, rows: int, size: int, out: torch.Tensor, scales: torch.Tensor) -> None:
         if rows and not size:
             raise KernelError(f"{what}: the rows have no values")
-        self._operand(what, "out", out, (torch.float8_e4m3fn,), (rows, size))
-        self._operand(what, "scales", scales, (torch.float32,), (rows,), dense=True)
-        if rows > 1 and out.stride(0) < size:
-            raise KernelError(f"{what}: the rows of out lie over one another")
-        self._apart(what, out, scales, *read)
-        self._apart(what, scales, *read)
+        self._operand(what, "out", out, _E4M3, (rows, size))
+        self._operand(what, "scales", scales, _FLOAT, (rows,), dense=True)
 
     def rmsnorm_e4m3(self, x: torch.Tensor, gain: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
                      delta: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None):
         """t = x + delta (written to `total`, or back to x where there is none), h = t / sqrt(mean(t^2) + eps) * gain, and h as 8-bit
         rows: scales[i] = max(max |h_i|, 2^-100) / 448, out[i] = h_i / scales[i] in float8_e4m3fn.  x and `total` 32-bit [T, D]; `delta`
-        and `gain` 32-bit or bfloat16.  A row that holds a NaN or an infinity gets a scale that is no finite number.  Returns (out, scales)."""
-        what, both = "rmsnorm_e4m3", (torch.float32, torch.bfloat16)
-        rows, size = self._operand(what, "x", x, (torch.float32,), (None, None), dense=True).shape
-        self._operand(what, "gain", gain, both, (size,), dense=True)
+        and `gain` 32-bit or bfloat16; all without gaps.  A row that holds a NaN or an infinity gets a scale that is no finite number.
+        Returns (out, scales)."""
+        what = "rmsnorm_e4m3"
+        rows, size = self._operand(what, "x", x, _FLOAT, dense=True).shape
+        self._operand(what, "gain", gain, _FLOATS, (size,), dense=True)
         if not eps > 0.0:
             raise KernelError(f"{what}: eps must be positive, got {eps}")
         if delta is not None:
-            self._operand(what, "delta", delta, both, (rows, size), dense=True)
-            if total is None or total is x:
+            self._operand(what, "delta", delta, _FLOATS, (rows, size), dense=True)
+            if total is None:
                 total = x
-            else:
-                self._apart(what, self._operand(what, "total", total, (torch.float32,), (rows, size), dense=True), x, gain, delta)
-            if total is x:
-                self._apart(what, x, delta, gain)
+            elif total is not x:
+                self._operand(what, "total", total, _FLOAT, (rows, size), dense=True)
         elif total is not None:
             raise KernelError(f"{what}: without a delta there is no sum to write")
-        self._quantised_places(what, rows, size, out, scales, x, gain, delta, total)
-        self._operand(what, "out", out, (torch.float8_e4m3fn,), dense=True)
+        self._operand(what, "out", out, _E4M3, (rows, size), dense=True)
+        self._quantised_places(what, rows, size, out, scales)
         if rows:
-            self._launch("rows_e4m3", "llme_rmsnorm_e4m3", what, c_void_p(x.data_ptr()), c_void_p(_ptr(delta)),
-                         c_int(_code(delta.dtype) if delta is not None else 0), c_void_p(gain.data_ptr()), c_int(_code(gain.dtype)),
-                         c_void_p(_ptr(total)), c_void_p(out.data_ptr()), c_void_p(scales.data_ptr()), c_int(rows), c_int(size), c_float(eps))
+            fn = self._entry("rows_e4m3", "llme_rmsnorm_e4m3", c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float)
+            self._launch("rows_e4m3", what, fn, x.data_ptr(), _ptr(delta), _code(delta.dtype) if delta is not None else 0, gain.data_ptr(),
+                         _code(gain.dtype), _ptr(total), out.data_ptr(), scales.data_ptr(), rows, size, eps)
         return out, scales
 
     def rows_e4m3(self, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
         """The rows of x [T, D] (32-bit or bfloat16, any row stride) as 8-bit rows: scales[i] = max(max |x_i|, 2^-100) / 448,
         out[i] = x_i / scales[i] in float8_e4m3fn (any row stride).  Returns (out, scales)."""
         what = "rows_e4m3"
-        rows, size = self._operand(what, "x", x, (torch.float32, torch.bfloat16), (None, None)).shape
-        if rows > 1 and x.stride(0) < size:
-            raise KernelError(f"{what}: the rows of x lie over one another")
-        self._quantised_places(what, rows, size, out, scales, x)
+        rows, size = self._operand(what, "x", x, _FLOATS).shape
+        self._quantised_places(what, rows, size, out, scales)
         if rows:
-            self._launch("rows_e4m3", "llme_rows_e4m3", what, c_void_p(x.data_ptr()), c_int(_code(x.dtype)), c_longlong(self._row_stride(x)),
-                         c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)), c_void_p(scales.data_ptr()), c_int(rows), c_int(size))
+            fn = self._entry("rows_e4m3", "llme_rows_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int)
+            self._launch("rows_e4m3", what, fn, x.data_ptr(), _code(x.dtype), self._row_stride(x), out.data_ptr(), self._row_stride(out),
+                         scales.data_ptr(), rows, size)
         return out, scales
 
     def swiglu_e4m3(self, gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
         """silu(gate) * up of gate_up [T, 2 D] = [gate | up] (32-bit or bfloat16, any row stride) as 8-bit rows, as `rows_e4m3` makes
         them.  Returns (out, scales)."""
         what = "swiglu_e4m3"
-        rows, both = self._operand(what, "gate_up", gate_up, (torch.float32, torch.bfloat16), (None, None)).shape
+        rows, both = self._operand(what, "gate_up", gate_up, _FLOATS).shape
         if both % 2:
             raise KernelError(f"{what}: gate_up must have an even number of columns, got {both}")
-        if rows > 1 and gate_up.stride(0) < both:
-            raise KernelError(f"{what}: the rows of gate_up lie over one another")
-        self._quantised_places(what, rows, both // 2, out, scales, gate_up)
+        self._quantised_places(what, rows, both // 2, out, scales)
         if rows:
-            self._launch("rows_e4m3", "llme_swiglu_e4m3", what, c_void_p(gate_up.data_ptr()), c_int(_code(gate_up.dtype)),
-                         c_longlong(self._row_stride(gate_up)), c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)),
-                         c_void_p(scales.data_ptr()), c_int(rows), c_int(both // 2))
+            fn = self._entry("rows_e4m3", "llme_swiglu_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int)
+            self._launch("rows_e4m3", what, fn, gate_up.data_ptr(), _code(gate_up.dtype), self._row_stride(gate_up), out.data_ptr(),
+                         self._row_stride(out), scales.data_ptr(), rows, both // 2)
         return out, scales
 
     # ------------------------------------------------------------------ products with weights of 8 and 4 bits
-    def _product_places(self, what: str, x: torch.Tensor, n: int, out: torch.Tensor, dtypes, *read: Optional[torch.Tensor]) -> None:
+    def _product_places(self, what: str, x: torch.Tensor, n: int, out: torch.Tensor, dtypes) -> None:
         rows = x.shape[0]
         self._operand(what, "out", out, dtypes, (rows, n))
-        for name, t in (("x", x), ("out", out)):
-            if rows > 1 and t.stride(0) < t.shape[1]:
-                raise KernelError(f"{what}: the rows of {name} lie over one another")
-        self._apart(what, out, x, *read)
 
     def linear_e4m3(self, x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """out[m, n] = x_scales[m] w_scales[n] (x[m] . w[n]) for x [M, K] and w [N, K] in float8_e4m3fn, scales 32-bit, out [M, N] 32-bit
         or bfloat16; sums are 32-bit.  K is a multiple of 16, the rows of x and w begin on 16 bytes (any such row stride)."""
-        what, f8 = "linear_e4m3", (torch.float8_e4m3fn,)
-        M, K = self._operand(what, "x", x, f8, (None, None)).shape
-        N = self._operand(what, "w", w, f8, (None, K)).shape[0]
-        self._operand(what, "x_scales", x_scales, (torch.float32,), (M,), dense=True)
-        self._operand(what, "w_scales", w_scales, (torch.float32,), (N,), dense=True)
-        self._product_places(what, x, N, out, (torch.float32, torch.bfloat16), w, x_scales, w_scales)
+        what = "linear_e4m3"
+        M, K = self._operand(what, "x", x, _E4M3).shape
+        N, Kw = self._operand(what, "w", w, _E4M3).shape
+        if Kw != K:
+            raise KernelError(f"{what}: rows of {K} values and weight rows of {Kw}")
+        self._operand(what, "x_scales", x_scales, _FLOAT, (M,), dense=True)
+        self._operand(what, "w_scales", w_scales, _FLOAT, (N,), dense=True)
+        self._product_places(what, x, N, out, _FLOATS)
         if M and N:
-            self._launch("gemm_e4m3", "llme_gemm_e4m3", what, c_void_p(x.data_ptr()), c_longlong(self._row_stride(x)), c_void_p(x_scales.data_ptr()),
-                         c_void_p(w.data_ptr()), c_longlong(self._row_stride(w)), c_void_p(w_scales.data_ptr()), c_void_p(out.data_ptr()),
-                         c_int(_code(out.dtype)), c_longlong(self._row_stride(out)), c_int(M), c_int(N), c_int(K))
+            fn = self._entry("gemm_e4m3", "llme_gemm_e4m3", c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int)
+            self._launch("gemm_e4m3", what, fn, x.data_ptr(), self._row_stride(x), x_scales.data_ptr(), w.data_ptr(), self._row_stride(w),
+                         w_scales.data_ptr(), out.data_ptr(), _code(out.dtype), self._row_stride(out), M, N, K)
         return out
 
     @staticmethod
@@ -692,17 +682,21 @@ class CudaOps:
         group of 32, 64 or 128; zeros uint8 of that shape with values 0..15 (None: 8 everywhere).  Sums are 32-bit.  K is a multiple
         of 8, the rows of x and w begin on 16 bytes (any such row stride)."""
         what = "linear_int4"
-        M, K = self._operand(what, "x", x, (torch.bfloat16,), (None, None)).shape
-        N = self._operand(what, "w", w, (torch.uint8,), (None, -(-K // 128) * 64)).shape[0]
-        groups = self._operand(what, "scales", scales, (torch.bfloat16,), (N, None), dense=True).shape[1]
+        M, K = self._operand(what, "x", x, _BF16S).shape
+        N, width = self._operand(what, "w", w, _BYTES).shape
+        if width != -(-K // 128) * 64:
+            raise KernelError(f"{what}: {K} codes a row take {-(-K // 128) * 64} bytes, w has {width}")
+        rows, groups = self._operand(what, "scales", scales, _BF16S, dense=True).shape
+        if rows != N:
+            raise KernelError(f"{what}: {N} weight rows and scales for {rows}")
         if zeros is not None:
-            self._operand(what, "zeros", zeros, (torch.uint8,), (N, groups), dense=True)
+            self._operand(what, "zeros", zeros, _BYTES, (N, groups), dense=True)
         group = self.int4_group(K, groups)
-        self._product_places(what, x, N, out, (torch.bfloat16,), w, scales, zeros)
+        self._product_places(what, x, N, out, _BF16S)
         if M and N:
-            self._launch("gemm_int4", "llme_gemm_int4", what, c_void_p(x.data_ptr()), c_longlong(self._row_stride(x)), c_void_p(w.data_ptr()),
-                         c_longlong(self._row_stride(w)), c_void_p(scales.data_ptr()), c_void_p(_ptr(zeros)), c_longlong(groups), c_int(group),
-                         c_void_p(out.data_ptr()), c_longlong(self._row_stride(out)), c_int(M), c_int(N), c_int(K))
+            fn = self._entry("gemm_int4", "llme_gemm_int4", c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_int, c_int)
+            self._launch("gemm_int4", what, fn, x.data_ptr(), self._row_stride(x), w.data_ptr(), self._row_stride(w), scales.data_ptr(), _ptr(zeros),
+                         groups, group, out.data_ptr(), self._row_stride(out), M, N, K)
         return out
 
     def _run_one(self, record) -> None:

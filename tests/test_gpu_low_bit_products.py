@@ -274,3 +274,14 @@ def test_refusals(ops):
         with pytest.raises(KernelError):
             call()
             print("not refused:", i)
+    assert ops.launches == n
+
+
+def test_operands_side_by_side(ops):
+    """Rows and output in one buffer, column range beside column range."""
+    x, xs, w, ws = _whole_e4m3(9, 32, 64, seed=6)
+    both = torch.zeros(9, 64 + 32 * 4, dtype=torch.uint8, device=DEV)
+    both[:, :64] = x.view(torch.uint8)
+    out = both[:, 64:].view(torch.float32)
+    ops.linear_e4m3(both[:, :64].view(F8), xs, w, ws, out)
+    assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws)) and torch.equal(both[:, :64], x.view(torch.uint8))
