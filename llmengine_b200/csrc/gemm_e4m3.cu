@@ -8,6 +8,8 @@
 // 128-value chunks of K in turn, and their partial sums are added in a fixed order.
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "operands.cuh"
 
@@ -15,7 +17,9 @@ LLME_API const char* llme_last_error() { return llme_error_buffer(); }
 
 namespace {
 
-typedef __nv_bfloat16 bf16;
+#include "umma.cuh"
+#include "gemm_wide.cuh"
+
 constexpr int KC = 128;           // values (bytes) per chunk: two blocks of 64
 
 struct Args {
@@ -42,15 +46,15 @@ template <int MT, typename O, int UNROLL, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     __shared__ float red[WARPS][MT * 8][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MT * 8);
+    const int n0 = blockIdx.x * 16;
     const unsigned char* w0 = a.w + (size_t)min(n0 + r, a.N - 1) * a.ldw + quad * 16;        // (a row past the end is read, never stored)
     const unsigned char* w1 = a.w + (size_t)min(n0 + r + 8, a.N - 1) * a.ldw + quad * 16;
     const unsigned char* xr[MT];
     bool xok[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        xok[m] = m0 + m * 8 + r < a.M;
-        xr[m] = a.x + (size_t)(xok[m] ? m0 + m * 8 + r : 0) * a.ldx + quad * 16;
+        xok[m] = m * 8 + r < a.M;
+        xr[m] = a.x + (size_t)(xok[m] ? m * 8 + r : 0) * a.ldx + quad * 16;
     }
     float acc[MT][4] = {};
     const int chunks = (a.K + KC - 1) / KC;
@@ -87,7 +91,7 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
         for (int i = 0; i < 4; ++i) red[warp][m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
     __syncthreads();
     for (int i = threadIdx.x; i < MT * 8 * 16; i += WARPS * 32) {
-        const int tok = m0 + (i >> 4), row = n0 + (i & 15);
+        const int tok = (i >> 4), row = n0 + (i & 15);
         if (tok >= a.M || row >= a.N) continue;
         float v = red[0][i >> 4][i & 15];
 #pragma unroll
@@ -96,11 +100,26 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     }
 }
 
+// More tokens than the weight-streaming kernel takes at once.
+int launch_wide(const Args& a, int out_f32, cudaStream_t s) {
+    wide::Args g{};
+    g.out = a.out; g.ldo = a.ldo; g.out_f32 = out_f32;
+    g.M = a.M; g.N = a.N; g.K = a.K;
+    g.xs = a.xs; g.ws = a.ws;
+    g.vec_out = (uintptr_t)a.out % (out_f32 ? 16 : 8) == 0 && a.ldo % 4 == 0;
+    wide::shape<false>(g);
+    alignas(64) CUtensorMap mw, mx;
+    if (int rc = make_map(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, a.K, a.ldw, BM, wide::STEP)) return rc;
+    if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, a.K, a.ldx, g.nt, wide::STEP)) return rc;
+    return wide::launch<false, 4, false>(mw, mx, g, s);
+}
+
 template <typename O>
 int launch(const Args& a, cudaStream_t s) {
+    if (a.M > 16) return launch_wide(a, sizeof(O) == 4, s);
     const int groups = (a.N + 15) / 16;
     if (a.M <= 8) llme_launch(skinny_kernel<1, O, 4, 8>, dim3(groups), dim3(256), 0, s, a);
-    else llme_launch(skinny_kernel<2, O, 2, 8>, dim3(groups, (a.M + 15) / 16), dim3(256), 0, s, a);
+    else llme_launch(skinny_kernel<2, O, 2, 8>, dim3(groups), dim3(256), 0, s, a);
     LLME_LAUNCH_STATUS();
 }
 
@@ -117,9 +136,11 @@ LLME_API int llme_gemm_e4m3(const void* x, long long ldx, const float* xs, const
     if (ldo < N) LLME_REFUSE("gemm_e4m3: output row stride shorter than the row");
     if (meets(span(out, M, N, ldo, out_dtype == LLME_F32 ? 4 : 2), {span(x, M, K, ldx, 1), span(w, N, K, ldw, 1), span(xs, 1, M, M, 4), span(ws, 1, N, N, 4)}))
         LLME_REFUSE("gemm_e4m3: the output lies over an operand");
-    if ((M + 15) / 16 > 65535) LLME_REFUSE("gemm_e4m3: %d rows are too many for one launch", M);
     const Args a{(const unsigned char*)x, ldx, xs, (const unsigned char*)w, ldw, ws, out, ldo, M, N, K};
     if (out_dtype == LLME_F32) return launch<float>(a, stream);
     if (out_dtype == LLME_BF16) return launch<bf16>(a, stream);
     LLME_REFUSE("gemm_e4m3: unsupported output dtype %d", out_dtype);
 }
+
+// 0 if no bounded wait has given up since the last call (synchronises the device).
+LLME_API int llme_gemm_e4m3_status() { LLME_TAKE_STATUS(g_status); }

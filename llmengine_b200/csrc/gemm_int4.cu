@@ -12,6 +12,8 @@
 // its scale, in 32-bit, when the group ends: no weight is rounded.
 //
 // The reference's weight-only product has 8-bit blocks (src/runtime/kernels/cuda_kernels.cu:296-358); it has none of 4 bits.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "operands.cuh"
 
@@ -19,7 +21,9 @@ LLME_API const char* llme_last_error() { return llme_error_buffer(); }
 
 namespace {
 
-typedef __nv_bfloat16 bf16;
+#include "umma.cuh"
+#include "gemm_wide.cuh"
+
 constexpr int BLOCK_K = 128, BLOCK_BYTES = 64;
 
 struct Args {
@@ -58,7 +62,7 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     constexpr int GROUPS = 4 / RUNS;                        // groups of a block of 128 values
     __shared__ float red[WARPS][MT * 8][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MT * 8);
+    const int n0 = blockIdx.x * 16;
     const size_t row0 = min(n0 + r, a.N - 1), row1 = min(n0 + r + 8, a.N - 1);            // (a row past the end is read, never stored)
     const unsigned char* w0 = a.w + row0 * a.ldw + quad * 16;
     const unsigned char* w1 = a.w + row1 * a.ldw + quad * 16;
@@ -66,8 +70,8 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     bool xok[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        xok[m] = m0 + m * 8 + r < a.M;
-        xr[m] = a.x + (size_t)(xok[m] ? m0 + m * 8 + r : 0) * a.ldx + quad * 8;
+        xok[m] = m * 8 + r < a.M;
+        xr[m] = a.x + (size_t)(xok[m] ? m * 8 + r : 0) * a.ldx + quad * 8;
     }
     float acc[MT][4] = {};
     const int blocks = (a.K + BLOCK_K - 1) / BLOCK_K, groups = (a.K + 32 * RUNS - 1) / (32 * RUNS);
@@ -121,7 +125,7 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
         for (int i = 0; i < 4; ++i) red[warp][m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
     __syncthreads();
     for (int i = threadIdx.x; i < MT * 8 * 16; i += WARPS * 32) {
-        const int tok = m0 + (i >> 4), row = n0 + (i & 15);
+        const int tok = (i >> 4), row = n0 + (i & 15);
         if (tok >= a.M || row >= a.N) continue;
         float v = red[0][i >> 4][i & 15];
 #pragma unroll
@@ -130,11 +134,28 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     }
 }
 
+// More tokens than the weight-streaming kernel takes at once.
+template <int RUNS, bool ZEROS>
+int launch_wide(const Args& a, cudaStream_t s) {
+    wide::Args g{};
+    g.out = a.out; g.ldo = a.ldo;
+    g.M = a.M; g.N = a.N; g.K = a.K;
+    g.scales = a.scales; g.zeros = a.zeros; g.lds = a.lds;
+    g.vec_out = (uintptr_t)a.out % 8 == 0 && a.ldo % 4 == 0;
+    wide::shape<true>(g);
+    const long long w_bytes = (a.K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES;
+    alignas(64) CUtensorMap mw, mx;
+    if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+    if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, g.nt, 64)) return rc;
+    return wide::launch<true, RUNS, ZEROS>(mw, mx, g, s);
+}
+
 template <int RUNS, bool ZEROS>
 int launch(const Args& a, cudaStream_t s) {
+    if (a.M > 16) return launch_wide<RUNS, ZEROS>(a, s);
     const int rows = (a.N + 15) / 16;
     if (a.M <= 8) llme_launch(skinny_kernel<1, RUNS, ZEROS, 4, 8>, dim3(rows), dim3(256), 0, s, a);
-    else llme_launch(skinny_kernel<2, RUNS, ZEROS, 2, 8>, dim3(rows, (a.M + 15) / 16), dim3(256), 0, s, a);
+    else llme_launch(skinny_kernel<2, RUNS, ZEROS, 2, 8>, dim3(rows), dim3(256), 0, s, a);
     LLME_LAUNCH_STATUS();
 }
 template <int RUNS>
@@ -158,9 +179,11 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     const long long groups = (K + group - 1LL) / group;
     if (meets(span(out, M, N, ldo, 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
         LLME_REFUSE("gemm_int4: the output lies over an operand");
-    if ((M + 15) / 16 > 65535) LLME_REFUSE("gemm_int4: %d rows are too many for one launch", M);
     const Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K};
     if (group == 32) return launch<1>(a, stream);
     if (group == 64) return launch<2>(a, stream);
     return launch<4>(a, stream);
 }
+
+// 0 if no bounded wait has given up since the last call (synchronises the device).
+LLME_API int llme_gemm_int4_status() { LLME_TAKE_STATUS(g_status); }
