@@ -29,6 +29,8 @@ struct Args {
     int M, N, K;
 };
 
+#include "gemm_e4m3_pair.cuh"
+
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -100,14 +102,21 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
     }
 }
 
-// More tokens than the weight-streaming kernel takes at once.
-int launch_wide(const Args& a, int out_f32, cudaStream_t s) {
+// More tokens than the weight-streaming kernel takes at once: 256 x 256 tiles on pairs of SMs, or narrower tiles with K cut over a cluster,
+// whichever a model of its time says is faster.  A step of 128 values takes a pair 580 cycles, starting and the last tile some 11,000
+// (64 x 4096 x 4096 / 12288: 16.2 / 34.2 us).
+template <typename O>
+int launch_wide(const Args& a, cudaStream_t s) {
+    constexpr int out_f32 = sizeof(O) == 4;
     wide::Args g{};
     g.out = a.out; g.ldo = a.ldo; g.out_f32 = out_f32;
     g.M = a.M; g.N = a.N; g.K = a.K;
     g.xs = a.xs; g.ws = a.ws;
     g.vec_out = (uintptr_t)a.out % (out_f32 ? 16 : 8) == 0 && a.ldo % 4 == 0;
-    wide::shape<false>(g);
+    double cycles;
+    if (int rc = wide::shape<false, 4, false>(g, &cycles)) return rc;
+    const long long pairs = sm_count() / 2, tiles = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
+    if ((double)((tiles + pairs - 1) / pairs) * ((a.K + 127) / 128) * 580.0 + 11000.0 < cycles) return pair::launch<O>(a, s);
     alignas(64) CUtensorMap mw, mx;
     if (int rc = make_map(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, a.K, a.ldw, BM, wide::STEP)) return rc;
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, a.K, a.ldx, g.nt, wide::STEP)) return rc;
@@ -116,7 +125,7 @@ int launch_wide(const Args& a, int out_f32, cudaStream_t s) {
 
 template <typename O>
 int launch(const Args& a, cudaStream_t s) {
-    if (a.M > 16) return launch_wide(a, sizeof(O) == 4, s);
+    if (a.M > 16) return launch_wide<O>(a, s);
     const int groups = (a.N + 15) / 16;
     if (a.M <= 8) llme_launch(skinny_kernel<1, O, 4, 8>, dim3(groups), dim3(256), 0, s, a);
     else llme_launch(skinny_kernel<2, O, 2, 8>, dim3(groups), dim3(256), 0, s, a);

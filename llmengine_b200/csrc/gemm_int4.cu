@@ -142,7 +142,7 @@ int launch_wide(const Args& a, cudaStream_t s) {
     g.M = a.M; g.N = a.N; g.K = a.K;
     g.scales = a.scales; g.zeros = a.zeros; g.lds = a.lds;
     g.vec_out = (uintptr_t)a.out % 8 == 0 && a.ldo % 4 == 0;
-    wide::shape<true>(g);
+    if (int rc = wide::shape<true, RUNS, ZEROS>(g, nullptr)) return rc;
     const long long w_bytes = (a.K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES;
     alignas(64) CUtensorMap mw, mx;
     if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;

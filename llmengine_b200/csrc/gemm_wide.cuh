@@ -15,12 +15,12 @@
 namespace wide {
 
 constexpr int STEP = 128;                        // values of K a stage holds
-constexpr int WORKERS = 8, PRODUCER = 8, ISSUER = 9, BLOCK = (WORKERS + 2) * 32, MOST_STAGES = 8;
-constexpr size_t MOST_SMEM = 232448;
+constexpr int WORKERS = 8, PRODUCER = 8, ISSUER = 9, BLOCK = (WORKERS + 2) * 32, MOST_STAGES = 8, MOST_SEGMENTS = 8;
+constexpr size_t MOST_SMEM = 232448, HALF_SMEM = 115712;      // of a block that has an SM to itself; of one of two (1 KB each is the system's)
 
 struct Args {
     void* out; long long ldo; int out_f32;
-    int M, N, K, nt, segments, segment_steps, stages, d_cols, vec_out;
+    int M, N, K, nt, segments, segment_steps, stages, d_cols, tmem_cols, per_sm, vec_out;
     const float* xs; const float* ws;                                                      // 8 bits
     const bf16* scales; const unsigned char* zeros; long long lds;                         // 4 bits
 };
@@ -29,6 +29,16 @@ struct Barriers {
     unsigned long long full[MOST_STAGES], ready[MOST_STAGES], done[MOST_STAGES], acc;
     unsigned tmem_base;
     int abort_flag;
+};
+
+// A stage and how often the ring has come round (a division by the number of stages takes longer than much of a step).
+struct Ring {
+    int stages, stage = 0;
+    unsigned phase = 0;
+    __device__ __forceinline__ explicit Ring(int n) : stages(n) {}
+    __device__ __forceinline__ void next() {
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
 };
 
 __device__ __forceinline__ bool elect_one() {
@@ -56,6 +66,10 @@ __device__ __forceinline__ void tmem_load8(unsigned addr, unsigned (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(addr));
 }
+// A request to bring a box into L2: it holds nothing back and may come ahead of what is written there.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void store_value(const Args& g, long long m, int n, float v) {
     if (g.out_f32) reinterpret_cast<float*>(g.out)[m * g.ldo + n] = v;
     else reinterpret_cast<bf16*>(g.out)[m * g.ldo + n] = __float2bfloat16_rn(v);
@@ -80,9 +94,8 @@ struct Group {
 
 // INT4: bfloat16 tokens and 4-bit weights; else both e4m3.
 template <bool INT4, int RUNS, bool ZEROS>
-__global__ void __launch_bounds__(BLOCK, 1)
+__global__ void __launch_bounds__(BLOCK, 2)
 wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args g) {
-    constexpr unsigned TMEM = INT4 ? 512 : 256;
     constexpr int W_BYTES = INT4 ? BM * STEP / 2 : BM * STEP;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -100,7 +113,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(&bar->full[s], 1);
-            mbar_init(&bar->ready[s], 4);
+            mbar_init(&bar->ready[s], 5);                          // four warps of a set, and the copy of the tokens' rows
             mbar_init(&bar->done[s], 1);
         }
         mbar_init(&bar->acc, 1);
@@ -108,37 +121,48 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == ISSUER) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(TMEM));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(g.tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = bar->tmem_base, tmem_w = tmem + (unsigned)g.d_cols;        // the accumulator; 64 columns of weights a stage
+    // (The kernel before may write what is taken for weights here: ahead of it goes only a request to have the first ones in L2.)
+    if (warp == PRODUCER && elect_one())
+        for (int c = 0; c < min(stages, steps); ++c) tma_prefetch_2d(&map_w, (step0 + c) * (INT4 ? STEP / 2 : STEP), n0);
+    __syncwarp();
     pdl_wait();
+    pdl_launch_dependents();        // (a block of the next kernel comes in when a block of this one has left its shared memory)
 
     if (warp == PRODUCER) {
+        Ring at(stages);
         int c = 0;
-        for (; c < steps; ++c) {
-            const int s = c % stages;
-            if (!mbar_wait(&bar->done[s], ((unsigned)(c / stages) & 1) ^ 1, abort_flag, 1) || *abort_flag) break;
+        for (; c < steps; ++c, at.next()) {
+            const int s = at.stage;
+            if (!mbar_wait(&bar->done[s], at.phase ^ 1, abort_flag, 1) || *abort_flag) break;
             if (elect_one()) {
-                mbar_expect_tx(&bar->full[s], W_BYTES + x_bytes);
+                // (4-bit weights: the tokens' bytes are counted where the numbers made of the codes are, for the instructions wait there)
+                unsigned long long* x_full = INT4 ? &bar->ready[s] : &bar->full[s];
+                mbar_expect_tx(&bar->full[s], INT4 ? W_BYTES : W_BYTES + x_bytes);
                 tma_load_2d(w_tiles + s * W_BYTES, &map_w, (step0 + c) * (INT4 ? STEP / 2 : STEP), n0, &bar->full[s]);
-                tma_load_2d(x_tiles + s * x_bytes, &map_x, (step0 + c) * STEP, m0, &bar->full[s]);
-                if (INT4) tma_load_2d(x_tiles + s * x_bytes + x_bytes / 2, &map_x, (step0 + c) * STEP + 64, m0, &bar->full[s]);
+                if (INT4) mbar_expect_tx(x_full, x_bytes);
+                tma_load_2d(x_tiles + s * x_bytes, &map_x, (step0 + c) * STEP, m0, x_full);
+                if (INT4) tma_load_2d(x_tiles + s * x_bytes + x_bytes / 2, &map_x, (step0 + c) * STEP + 64, m0, x_full);
             }
             __syncwarp();
         }
-        if (c < steps)                                             // gave up: the copies that may still be in flight land first
+        if (c < steps) {                                           // gave up: the copies that may still be in flight land first
             for (int j = max(0, c - stages); j < c; ++j)
                 for (unsigned n = 0; n < WAIT_LIMIT && !mbar_try_wait(&bar->full[j % stages], (unsigned)(j / stages) & 1); ++n) {}
+            if (INT4) for (int i = 0; i < 200; ++i) __nanosleep(5000);         // (the tokens' barriers may lack an arrival: far longer than a copy takes)
+        }
     } else if (warp == ISSUER) {
         const unsigned id = INT4 ? umma_idesc(BM, nt) : idesc_e4m3(BM, nt);
-        for (int c = 0; c < steps; ++c) {
-            const int s = c % stages;
-            if (!mbar_wait(&bar->full[s], (unsigned)(c / stages) & 1, abort_flag, 2)) break;
-            if (INT4 && !mbar_wait(&bar->ready[s], (unsigned)(c / stages) & 1, abort_flag, 3)) break;
+        Ring at(stages);
+        for (int c = 0; c < steps; ++c, at.next()) {
+            const int s = at.stage;
+            if (!mbar_wait(INT4 ? &bar->ready[s] : &bar->full[s], at.phase, abort_flag, 2)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one()) {
                 const unsigned long long x = umma_desc(x_tiles + s * x_bytes);
@@ -166,11 +190,13 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         const unsigned mine = tmem_w + ((unsigned)(quarter * 32) << 16);
         Group<RUNS, ZEROS> next;
         next.fetch(scales, zeros, step0 + set, groups);
-        for (int c = set; c < steps; c += 2) {
-            const int s = c % stages;
+        Ring at(stages);
+        if (set) at.next();
+        for (int c = set; c < steps; c += 2, at.next(), at.next()) {
+            const int s = at.stage;
             const Group<RUNS, ZEROS> now = next;
             next.fetch(scales, zeros, step0 + c + 2, groups);
-            if (!mbar_wait(&bar->full[s], (unsigned)(c / stages) & 1, abort_flag, 4)) break;
+            if (!mbar_wait(&bar->full[s], at.phase, abort_flag, 4)) break;
             // unit q holds word 4 q + j; the 64-byte swizzle put it at q ^ (row / 2 % 4), so that eight lanes meet no bank twice
             const unsigned char* src = w_tiles + s * W_BYTES + row * 64;
             unsigned words[4][4];
@@ -198,7 +224,6 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         }
     }
     __syncwarp();
-    pdl_launch_dependents();                                       // the next kernel may be scheduled while the sums are put together
     float* part = reinterpret_cast<float*>(smem);                  // [token][128 weight rows]
     if (warp < WORKERS) {
         const int row = quarter * 32 + lane, n = n0 + row, half = nt / 2, col0 = (warp >> 2) * half;
@@ -226,7 +251,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     __syncthreads();
     if (warp == ISSUER) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols));
     }
     if (g.segments == 1) return;
     cluster_sync();
@@ -235,13 +260,17 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     for (int e = rank * BLOCK + (int)threadIdx.x; e < nt * (BM / 4); e += g.segments * BLOCK) {
         const int m = m0 + e / (BM / 4), n = n0 + (e % (BM / 4)) * 4;
         if (m >= g.M || n >= g.N) continue;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int from = 0; from < g.segments; ++from) {
-            float4 f;
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(map_to_cta(from_here + 16u * (unsigned)e, (unsigned)from)) : "memory");
-            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-        }
+        // (all of a place's loads are under way before the first is added: one after the other each takes some 700 cycles)
+        float4 f[MOST_SEGMENTS];
+#pragma unroll
+        for (int from = 0; from < MOST_SEGMENTS; ++from)
+            if (from < g.segments)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(f[from].x), "=f"(f[from].y), "=f"(f[from].z), "=f"(f[from].w) : "r"(map_to_cta(from_here + 16u * (unsigned)e, (unsigned)from)));
+        float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+        for (int from = 1; from < MOST_SEGMENTS; ++from)
+            if (from < g.segments) { v[0] += f[from].x; v[1] += f[from].y; v[2] += f[from].z; v[3] += f[from].w; }
         if (!INT4) {
             const float xs = g.xs[m];
 #pragma unroll
@@ -281,37 +310,76 @@ int make_map_swizzled(CUtensorMap* map, const void* base, CUtensorMapDataType ty
     return 0;
 }
 
-// Tile width, segments and stages of a product.  A step costs a block the longest of its instructions (nt cycles for 128 e4m3 values twice,
-// four times nt for bfloat16) and of what it brings, at some 40 bytes a cycle where all SMs read; starting and ending cost about 4,000
-// cycles, the cluster's sums 2,000 and a little for every token.
-template <bool INT4>
-void shape(Args& g) {
-    const int steps = (g.K + STEP - 1) / STEP, n_tiles = (g.N + BM - 1) / BM, w_bytes = INT4 ? BM * STEP / 2 : BM * STEP;
-    const int widest = 256, least = (g.M + widest - 1) / widest;
+// How many clusters of `segments` blocks the GPU holds at once, `per_sm` blocks an SM: a cluster's blocks need SMs of one GPC, and what is
+// left of a GPC stays empty.  (Asked once for every size of cluster.)
+template <bool INT4, int RUNS, bool ZEROS>
+int clusters_held(int segments, int per_sm) {
+    static std::atomic<int> known[2][MOST_SEGMENTS + 1];
+    std::atomic<int>& one = known[per_sm - 1][segments];
+    int n = one.load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024, 1, segments);
+    cfg.blockDim = dim3(BLOCK);
+    cfg.dynamicSmemBytes = per_sm == 1 ? MOST_SMEM : HALF_SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = (unsigned)segments;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const int all = per_sm * sm_count() / segments;
+    if (segments == 1 || cudaOccupancyMaxActiveClusters(&n, wide_kernel<INT4, RUNS, ZEROS>, &cfg) != cudaSuccess || n <= 0 || n > all) {
+        cudaGetLastError();
+        n = all;
+    }
+    one.store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// Tile width, segments, blocks an SM and stages of a product: what a model of its time says is least, in cycles.  The blocks that run at once
+// (as many as are held) share the memory's 2,900 bytes a cycle for the weights; an SM's blocks share its 42 bytes a cycle from L2 and its
+// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16).  Starting and ending a block cost about 5,500
+// cycles, the cluster's sums 1,000 and a little for every token.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
+// 19.2 us, both in segments of four.)
+template <bool INT4, int RUNS, bool ZEROS>
+int shape(Args& g, double* cycles) {
+    const int steps = (g.K + STEP - 1) / STEP, n_tiles = (g.N + BM - 1) / BM, w_bytes = INT4 ? BM * STEP / 2 : BM * STEP, x_width = STEP * (INT4 ? 2 : 1);
+    const int least = (g.M + 255) / 256;
+    static LlmeGrants grants;
+    if (cudaError_t e = llme_grant_smem(grants, wide_kernel<INT4, RUNS, ZEROS>, MOST_SMEM)) LLME_REFUSE("gemm_wide: cannot reserve %zu bytes of shared memory: %s", MOST_SMEM, cudaGetErrorString(e));
     double best = -1.0;
     for (int m_tiles = least; m_tiles <= least + 3; ++m_tiles) {
-        const int nt = ((g.M + m_tiles - 1) / m_tiles + 15) / 16 * 16, tiles = n_tiles * ((g.M + nt - 1) / nt);
-        for (int segments = 1; segments <= 8 && segments <= steps; ++segments) {
-            const int each = (steps + segments - 1) / segments, used = (steps + each - 1) / each;
-            if (used != segments) continue;
-            const double rounds = (double)(((long long)tiles * segments + sm_count() - 1) / sm_count());
-            const double multiply = (INT4 ? 4.0 : 2.0) * nt, bring = (w_bytes + nt * STEP * (INT4 ? 2.0 : 1.0)) / 40.0;
-            const double cost = rounds * (each * (multiply > bring ? multiply : bring) + 4000.0 + (segments > 1 ? 2000.0 + 4.0 * nt : 0.0));
-            if (best < 0.0 || cost < best) { best = cost; g.nt = nt; g.segments = segments; g.segment_steps = each; }
-        }
+        const int nt = ((g.M + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+        const long long tiles = (long long)n_tiles * ((g.M + nt - 1) / nt);
+        for (int per_sm = 1; per_sm <= (nt <= 64 ? 2 : 1); ++per_sm)
+            for (int segments = 1; segments <= MOST_SEGMENTS && segments <= steps; ++segments) {
+                const int each = (steps + segments - 1) / segments;
+                if ((steps + each - 1) / each != segments) continue;
+                const int held = clusters_held<INT4, RUNS, ZEROS>(segments, per_sm);
+                const double rounds = (double)((tiles + held - 1) / held), at_once = (double)(tiles < held ? tiles : held) * segments;
+                const double share = at_once > sm_count() ? at_once / sm_count() : 1.0;                   // blocks on an SM
+                double step = share * (INT4 ? 4.0 : 2.0) * nt;
+                if (step < share * (w_bytes + nt * x_width) / 42.0) step = share * (w_bytes + nt * x_width) / 42.0;
+                if (step < at_once * w_bytes / 2900.0) step = at_once * w_bytes / 2900.0;
+                const double cost = rounds * (each * step + 5500.0 + (segments > 1 ? 1000.0 + 4.0 * nt : 0.0));
+                if (best < 0.0 || cost < best) { best = cost; g.nt = nt; g.segments = segments; g.segment_steps = each; g.per_sm = per_sm; }
+            }
     }
     g.d_cols = g.nt <= 64 ? 64 : (g.nt <= 128 ? 128 : 256);
-    const int stage = w_bytes + g.nt * STEP * (INT4 ? 2 : 1), fit = (int)((MOST_SMEM - 1024 - sizeof(Barriers)) / stage);
+    g.tmem_cols = INT4 && g.per_sm == 1 ? 512 : 256;
+    const int fit = (int)(((g.per_sm == 1 ? MOST_SMEM : HALF_SMEM) - 1024 - sizeof(Barriers)) / (w_bytes + g.nt * x_width));
     g.stages = fit < MOST_STAGES ? fit : MOST_STAGES;
-    if (INT4 && g.stages > (512 - g.d_cols) / 64) g.stages = (512 - g.d_cols) / 64;
+    if (INT4 && g.stages > (g.tmem_cols - g.d_cols) / 64) g.stages = (g.tmem_cols - g.d_cols) / 64;
+    if (cycles) *cycles = best;
+    return 0;
 }
 
 template <bool INT4, int RUNS, bool ZEROS>
 int launch(const CUtensorMap& mw, const CUtensorMap& mx, const Args& g, cudaStream_t stream) {
     const size_t smem = 1024 + (size_t)g.stages * ((INT4 ? BM * STEP / 2 : BM * STEP) + (size_t)g.nt * STEP * (INT4 ? 2 : 1)) + sizeof(Barriers);
     auto kernel = wide_kernel<INT4, RUNS, ZEROS>;
-    static LlmeGrants grants;
-    if (cudaError_t e = llme_grant_smem(grants, kernel, MOST_SMEM)) LLME_REFUSE("gemm_wide: cannot reserve %zu bytes of shared memory: %s", MOST_SMEM, cudaGetErrorString(e));
     const long long blocks = (long long)((g.M + g.nt - 1) / g.nt) * ((g.N + BM - 1) / BM);
     if (blocks > 2147483647LL) LLME_REFUSE("gemm_wide: %d x %d outputs are too many for one launch", g.M, g.N);
     cudaLaunchConfig_t cfg = {};
