@@ -1,11 +1,11 @@
 // out[M,N] = xs[m] ws[n] (x[M,K] * W[N,K]^T) with x and W in 8-bit floating point (e4m3) and one 32-bit scale for every row of x and
 // of W: the product of a layer whose weights and activations are 8-bit.  Sums are 32-bit, the scales multiply the finished sum.
 //
-// A handful of tokens: bound by reading W once.  16 rows of W are the M side of a mma.sync.m16n8k32 tile and the tokens its N side.
-// The order in which the k values of a dot product are added is free: within every 64 values the four lanes of a quad take 16
-// consecutive ones each, for W and x alike, so that a lane's operands for two steps are one 16-byte load of a row of W (two rows a
-// lane) and one of a row of x, straight into the registers the instruction reads.  A block owns 16 rows of W, its warps take the
-// 128-value chunks of K in turn, and their partial sums are added in a fixed order.
+// Up to 16 tokens: bound by reading W once.  16 rows of W are the M side of a mma.sync.m16n8k32 tile and the tokens its N side.  The
+// order in which the k values of a dot product are added is free: within every 64 values the four lanes of a quad take 16 consecutive ones
+// each, for W and x alike, so that a lane's operands for two steps are 16 bytes of a row of W (two rows a lane), on their way through a ring
+// in shared memory (weight_stream.cuh), and one 16-byte load of a row of x.
+// More: tcgen05, the weights on the lanes of tensor memory (gemm_wide.cuh) or 256 x 256 tiles on pairs of SMs (gemm_e4m3_pair.cuh).
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
 #include <cuda.h>
@@ -19,8 +19,9 @@ namespace {
 
 #include "umma.cuh"
 #include "gemm_wide.cuh"
+#include "weight_stream.cuh"
 
-constexpr int KC = 128;           // values (bytes) per chunk: two blocks of 64
+constexpr int KC = stream::PIECE; // values (bytes) of a row in a step: two blocks of 64
 
 struct Args {
     const unsigned char* x; long long ldx; const float* xs;
@@ -36,70 +37,97 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], unsigned a0, unsigned a1
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// weights are read once: do not keep them in L1
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-// MT: 8-token tiles.  UNROLL: chunks of K whose loads a warp issues together.
-template <int MT, typename O, int UNROLL, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
-    __shared__ float red[WARPS][MT * 8][16];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2;
-    const int n0 = blockIdx.x * 16;
+// MT: 8-token tiles.  SHARE: warps that share a row group; AN_SM: warps an SM is to hold.
+template <int MT, typename O, int SHARE, int AN_SM>
+__global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args a) {
+    extern __shared__ __align__(128) unsigned char rings[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2, n0 = blockIdx.x * 16;
     const unsigned char* w0 = a.w + (size_t)min(n0 + r, a.N - 1) * a.ldw + quad * 16;        // (a row past the end is read, never stored)
     const unsigned char* w1 = a.w + (size_t)min(n0 + r + 8, a.N - 1) * a.ldw + quad * 16;
-    const unsigned char* xr[MT];
-    bool xok[MT];
+    // (lanes without a token read the first one: a token's sums are its own, and theirs are not stored)
+    const unsigned char* xp[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        xok[m] = m * 8 + r < a.M;
-        xr[m] = a.x + (size_t)(xok[m] ? m * 8 + r : 0) * a.ldx + quad * 16;
-    }
+    for (int m = 0; m < MT; ++m) xp[m] = a.x + (size_t)(m * 8 + r < a.M ? m * 8 + r : 0) * a.ldx + quad * 16 + warp * KC;
     float acc[MT][4] = {};
-    const int chunks = (a.K + KC - 1) / KC;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int pieces = (a.K + KC - 1) / KC;
+    const stream::Ring ring(rings);
+    // (The kernel before may write what is taken for weights here: ahead of it goes only a request to have the first ones in L2.)
+    if (quad == 0)
+        for (int i = 0, t = warp; i < stream::DEPTH - 1 && t < pieces; ++i, t += SHARE) { stream::prefetch_l2(w0 + (size_t)t * KC); stream::prefetch_l2(w1 + (size_t)t * KC); }
     pdl_wait();
     pdl_launch_dependents();
-    for (int c = warp; c < chunks; c += UNROLL * WARPS) {
-        uint4 wa[UNROLL][2], wb[UNROLL][2], xv[UNROLL][MT][2];
+    int ahead = warp;                                       // the piece that is brought next
+    w0 += (size_t)warp * KC;
+    w1 += (size_t)warp * KC;
+    auto bring = [&](int slot) {
+        // K is a multiple of 16: a lane's 16 bytes are inside or outside
+        if (ahead < pieces) ring.bring(slot, w0, w1, ahead * KC + quad * 16 < a.K, ahead * KC + 64 + quad * 16 < a.K);
+        stream::Ring::close();
+        ahead += SHARE;
+        w0 += SHARE * KC;
+        w1 += SHARE * KC;
+    };
 #pragma unroll
-        for (int q = 0; q < UNROLL; ++q)
+    for (int i = 0; i < stream::DEPTH - 1; ++i) bring(i);
+    int slot = 0;
+    for (int t = warp; t < pieces; t += SHARE) {
+        bring(slot == 0 ? stream::DEPTH - 1 : slot - 1);
+        uint4 xv[MT][2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int k = (c + q * WARPS) * KC + b * 64;
-                const bool ok = k + quad * 16 < a.K;              // K is a multiple of 16: a piece is inside or outside
-                wa[q][b] = ok ? load_stream(w0 + k) : zero;
-                wb[q][b] = ok ? load_stream(w1 + k) : zero;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) xv[q][m][b] = ok && xok[m] ? *reinterpret_cast<const uint4*>(xr[m] + k) : zero;
+            for (int m = 0; m < MT; ++m)
+                xv[m][b] = t * KC + b * 64 + quad * 16 < a.K ? *reinterpret_cast<const uint4*>(xp[m] + b * 64) : make_uint4(0u, 0u, 0u, 0u);
+        stream::Ring::wait();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            uint4 c0 = ring.read(slot, b, 0), c1 = ring.read(slot, b, 1);
+            // (behind K nothing was brought: what lies there may be no number)
+            if (t * KC + b * 64 + quad * 16 >= a.K) c0 = c1 = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                mma_e4m3(acc[m], c0.x, c1.x, c0.y, c1.y, xv[m][b].x, xv[m][b].y);
+                mma_e4m3(acc[m], c0.z, c1.z, c0.w, c1.w, xv[m][b].z, xv[m][b].w);
             }
+        }
+        slot = slot + 1 == stream::DEPTH ? 0 : slot + 1;
 #pragma unroll
-        for (int q = 0; q < UNROLL; ++q)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    mma_e4m3(acc[m], wa[q][b].x, wb[q][b].x, wa[q][b].y, wb[q][b].y, xv[q][m][b].x, xv[q][m][b].y);
-                    mma_e4m3(acc[m], wa[q][b].z, wb[q][b].z, wa[q][b].w, wb[q][b].w, xv[q][m][b].z, xv[q][m][b].w);
-                }
+        for (int m = 0; m < MT; ++m) xp[m] += SHARE * KC;
     }
-    // the warps' partial sums, added in a fixed order
+    // the sums of the warps that share a row group, added in their order
+    float (*red)[16] = reinterpret_cast<float (*)[16]>(rings);                     // [warp * 8 MT + token][row]: over the rings, which are empty now
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[warp][m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
+        for (int i = 0; i < 4; ++i) red[warp * MT * 8 + m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 8 * 16; i += WARPS * 32) {
-        const int tok = (i >> 4), row = n0 + (i & 15);
+    for (int i = threadIdx.x; i < MT * 8 * 16; i += SHARE * 32) {
+        const int tok = i >> 4, row = n0 + (i & 15);
         if (tok >= a.M || row >= a.N) continue;
-        float v = red[0][i >> 4][i & 15];
+        float v = red[tok][i & 15];
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) v += red[w][i >> 4][i & 15];
+        for (int w = 1; w < SHARE; ++w) v += red[w * MT * 8 + tok][i & 15];
         reinterpret_cast<O*>(a.out)[(size_t)tok * a.ldo + row] = from_f32<O>(v * a.xs[tok] * a.ws[row]);
     }
+}
+
+template <int MT, typename O, int SHARE, int AN_SM>
+int launch_skinny(const Args& a, cudaStream_t s) {
+    constexpr size_t smem = SHARE * stream::RING;
+    static_assert(MT * 8 * 16 * 4 <= stream::RING, "the sums lie over the rings");
+    auto kernel = skinny_kernel<MT, O, SHARE, AN_SM>;
+    static LlmeGrants grants;
+    if (cudaError_t e = llme_grant_smem(grants, kernel, smem)) LLME_REFUSE("gemm_e4m3: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    llme_launch(kernel, dim3((a.N + 15) / 16), dim3(SHARE * 32), smem, s, a);
+    LLME_LAUNCH_STATUS();
+}
+template <int MT, typename O>
+int launch_skinny(const Args& a, cudaStream_t s) {
+    stream::Shares by = stream::sharing((a.N + 15) / 16, (a.K + KC - 1) / KC, sm_count());
+    if (by.warps == 16) return launch_skinny<MT, O, 16, 16>(a, s);
+    if (by.warps == 8) return by.an_sm == 16 ? launch_skinny<MT, O, 8, 16>(a, s) : launch_skinny<MT, O, 8, 24>(a, s);
+    return by.warps == 4 ? launch_skinny<MT, O, 4, 24>(a, s) : launch_skinny<MT, O, 2, 24>(a, s);
 }
 
 // More tokens than the weight-streaming kernel takes at once: 256 x 256 tiles on pairs of SMs, or narrower tiles with K cut over a cluster,
@@ -126,10 +154,7 @@ int launch_wide(const Args& a, cudaStream_t s) {
 template <typename O>
 int launch(const Args& a, cudaStream_t s) {
     if (a.M > 16) return launch_wide<O>(a, s);
-    const int groups = (a.N + 15) / 16;
-    if (a.M <= 8) llme_launch(skinny_kernel<1, O, 4, 8>, dim3(groups), dim3(256), 0, s, a);
-    else llme_launch(skinny_kernel<2, O, 2, 8>, dim3(groups), dim3(256), 0, s, a);
-    LLME_LAUNCH_STATUS();
+    return a.M <= 8 ? launch_skinny<1, O>(a, s) : launch_skinny<2, O>(a, s);
 }
 
 }  // namespace

@@ -13,6 +13,7 @@
 //
 // The reference's weight-only product has 8-bit blocks (src/runtime/kernels/cuda_kernels.cu:296-358); it has none of 4 bits.
 #include <cuda.h>
+#include <type_traits>
 
 #include "common.cuh"
 #include "operands.cuh"
@@ -23,6 +24,7 @@ namespace {
 
 #include "umma.cuh"
 #include "gemm_wide.cuh"
+#include "weight_stream.cuh"
 
 constexpr int BLOCK_K = 128, BLOCK_BYTES = 64;
 
@@ -32,6 +34,7 @@ struct Args {
     const bf16* scales; const unsigned char* zeros; long long lds;      // values from row to row of both
     bf16* out; long long ldo;
     int M, N, K;
+    int vec_scales;                                         // a block's scales and zero points begin on their size
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -39,74 +42,128 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// weights are read once: do not keep them in L1
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+// A word's eight codes less the zero point, in the order of their values, as bfloat16 numbers of 2^-6: without a shift for half of them.  As
+// bits of a bfloat16 number a code in the low four bits is c 2^-133, and one in the next four 16 c 2^-133 (the numbers below 2^-125 all have
+// the same distance); the factors 2^127 and 2^123 make both c 2^-6, and the addend takes z 2^-6 off in the same instruction, exactly.
+// (Arithmetic bounds this kernel: a logical instruction, a shift and one on two bfloat16 numbers all take two cycles a warp.)
+__device__ __forceinline__ void eight_codes(unsigned word, __nv_bfloat162 minus_z, unsigned (&v)[4]) {
+    const unsigned up = word >> 8;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const unsigned code = (p < 2 ? word : up) & (p & 1 ? 0x00f000f0u : 0x000f000fu), factor = p & 1 ? 0x7d007d00u : 0x7f007f00u;
+        const __nv_bfloat162 w = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&code), *reinterpret_cast<const __nv_bfloat162*>(&factor), minus_z);
+        v[p] = *reinterpret_cast<const unsigned*>(&w);
+    }
+}
+// -z 2^-6, twice
+__device__ __forceinline__ __nv_bfloat162 minus_zero_point(unsigned z) { return __float2bfloat162_rn(-(float)z * 0.015625f); }
+
+// COUNT neighbouring scales (2 bytes each) or zero points (1 byte each) side by side in T, in one load where `whole` says that they begin on
+// their size.
+template <typename T, int COUNT, int BYTES>
+__device__ __forceinline__ T load_few(const unsigned char* p, bool whole) {
+    if (COUNT > 1 && whole) {
+        if constexpr (COUNT * BYTES == 2) return *reinterpret_cast<const unsigned short*>(p);
+        else if constexpr (COUNT * BYTES == 4) return *reinterpret_cast<const unsigned*>(p);
+        else if constexpr (COUNT * BYTES == 8) return (T)*reinterpret_cast<const unsigned long long*>(p);
+    }
+    T v = 0;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v |= (T)(BYTES == 1 ? (unsigned)p[i] : (unsigned)*reinterpret_cast<const unsigned short*>(p + 2 * i)) << (8 * BYTES * i);
     return v;
 }
-// codes 2p and 2p + 1 of a word as bfloat16 numbers minus z (`bias` holds 128 + z twice)
-__device__ __forceinline__ unsigned two_codes(unsigned word, int p, __nv_bfloat162 bias) {
-    const unsigned c = ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), bias);
-    return *reinterpret_cast<const unsigned*>(&v);
-}
-__device__ __forceinline__ __nv_bfloat162 bias_of(unsigned zero) {
-    const unsigned b = 0x43004300u | zero | zero << 16;
-    return *reinterpret_cast<const __nv_bfloat162*>(&b);
-}
 
-// MT: 8-token tiles.  RUNS: runs of 32 values in a group (1, 2 or 4).  UNROLL: blocks of 128 values whose loads a warp issues together.
-template <int MT, int RUNS, bool ZEROS, int UNROLL, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
-    constexpr int GROUPS = 4 / RUNS;                        // groups of a block of 128 values
-    __shared__ float red[WARPS][MT * 8][16];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2;
+// What goes with two rows' codes: the scales and zero points of a block of 128 values.
+template <int GROUPS, bool ZEROS>
+struct Factors {
+    typedef std::conditional_t<GROUPS == 4, unsigned long long, unsigned> S;
+    S s0, s1;
+    unsigned z0, z1;
+    __device__ __forceinline__ void fetch(const Args& a, const unsigned char* scales0, const unsigned char* scales1, size_t row0, size_t row1, int first, int groups) {
+        s0 = s1 = 0;                                        // (behind K there are no scales, and what they would multiply is zero)
+        z0 = z1 = 0;
+        if (first + GROUPS <= groups) {
+            s0 = load_few<S, GROUPS, 2>(scales0 + 2 * (size_t)first, a.vec_scales);
+            s1 = load_few<S, GROUPS, 2>(scales1 + 2 * (size_t)first, a.vec_scales);
+            if (ZEROS) {
+                z0 = load_few<unsigned, GROUPS, 1>(a.zeros + row0 * a.lds + first, a.vec_scales);
+                z1 = load_few<unsigned, GROUPS, 1>(a.zeros + row1 * a.lds + first, a.vec_scales);
+            }
+        } else if (GROUPS > 1) {
+            for (int g = 0; g < GROUPS && first + g < groups; ++g) {
+                s0 |= load_few<S, 1, 2>(scales0 + 2 * (size_t)(first + g), false) << (16 * g);
+                s1 |= load_few<S, 1, 2>(scales1 + 2 * (size_t)(first + g), false) << (16 * g);
+                if (ZEROS) {
+                    z0 |= load_few<unsigned, 1, 1>(a.zeros + row0 * a.lds + first + g, false) << (8 * g);
+                    z1 |= load_few<unsigned, 1, 1>(a.zeros + row1 * a.lds + first + g, false) << (8 * g);
+                }
+            }
+        }
+    }
+};
+
+// MT: 8-token tiles.  RUNS: runs of 32 values in a group (1, 2 or 4).  SHARE: warps that share a row group; AN_SM: warps an SM is to hold.
+template <int MT, int RUNS, bool ZEROS, int SHARE, int AN_SM>
+__global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args a) {
+    constexpr int GROUPS = 4 / RUNS, PAIR = 2 * BLOCK_K;          // a piece of 128 bytes is two blocks of codes
+    extern __shared__ __align__(128) unsigned char rings[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, r = lane >> 2, part = warp;
     const int n0 = blockIdx.x * 16;
     const size_t row0 = min(n0 + r, a.N - 1), row1 = min(n0 + r + 8, a.N - 1);            // (a row past the end is read, never stored)
     const unsigned char* w0 = a.w + row0 * a.ldw + quad * 16;
     const unsigned char* w1 = a.w + row1 * a.ldw + quad * 16;
-    const bf16* xr[MT];
-    bool xok[MT];
+    const unsigned char* scales0 = reinterpret_cast<const unsigned char*>(a.scales + row0 * a.lds);
+    const unsigned char* scales1 = reinterpret_cast<const unsigned char*>(a.scales + row1 * a.lds);
+    // (lanes without a token read the first one: a token's sums are its own, and theirs are not stored)
+    const bf16* xp[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        xok[m] = m * 8 + r < a.M;
-        xr[m] = a.x + (size_t)(xok[m] ? m * 8 + r : 0) * a.ldx + quad * 8;
-    }
+    for (int m = 0; m < MT; ++m) xp[m] = a.x + (size_t)(m * 8 + r < a.M ? m * 8 + r : 0) * a.ldx + quad * 8 + part * PAIR;
     float acc[MT][4] = {};
-    const int blocks = (a.K + BLOCK_K - 1) / BLOCK_K, groups = (a.K + 32 * RUNS - 1) / (32 * RUNS);
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int blocks = (a.K + BLOCK_K - 1) / BLOCK_K, pieces = (blocks + 1) / 2, groups = (a.K + 32 * RUNS - 1) / (32 * RUNS);
+    const stream::Ring ring(rings);
+    // (The kernel before may write what is taken for weights here: ahead of it goes only a request to have the first ones in L2.)
+    if (quad == 0)
+        for (int i = 0, t = part; i < stream::DEPTH - 1 && t < pieces; ++i, t += SHARE) { stream::prefetch_l2(w0 + (size_t)t * stream::PIECE); stream::prefetch_l2(w1 + (size_t)t * stream::PIECE); }
     pdl_wait();
     pdl_launch_dependents();
-    for (int c = warp; c < blocks; c += UNROLL * WARPS) {
-        uint4 wa[UNROLL], wb[UNROLL];
+    int ahead = part;                                       // the piece that is brought next
+    w0 += (size_t)part * stream::PIECE;
+    w1 += (size_t)part * stream::PIECE;
+    auto bring = [&](int slot) {
+        if (ahead < pieces) ring.bring(slot, w0, w1, true, 2 * ahead + 1 < blocks);
+        stream::Ring::close();
+        ahead += SHARE;
+        w0 += SHARE * stream::PIECE;
+        w1 += SHARE * stream::PIECE;
+    };
 #pragma unroll
-        for (int q = 0; q < UNROLL; ++q) {
-            const bool ok = c + q * WARPS < blocks;
-            wa[q] = ok ? load_stream(w0 + (size_t)(c + q * WARPS) * BLOCK_BYTES) : zero;
-            wb[q] = ok ? load_stream(w1 + (size_t)(c + q * WARPS) * BLOCK_BYTES) : zero;
-        }
+    for (int i = 0; i < stream::DEPTH - 1; ++i) bring(i);
+    Factors<GROUPS, ZEROS> next[2], now[2];
 #pragma unroll
-        for (int q = 0; q < UNROLL; ++q) {
-            const int block = c + q * WARPS;
-            if (block >= blocks) break;
-            const unsigned word0[4] = {wa[q].x, wa[q].y, wa[q].z, wa[q].w}, word1[4] = {wb[q].x, wb[q].y, wb[q].z, wb[q].w};
+    for (int b = 0; b < 2; ++b) next[b].fetch(a, scales0, scales1, row0, row1, (2 * part + b) * GROUPS, groups);
+    // a piece's products; `last`: the piece in which K ends
+    auto multiply = [&](int slot, int t, auto last) {
+        constexpr bool LAST = decltype(last)::value;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            // (the second block of the last piece may not be there: whatever codes lie in its place meet zeros)
+            const uint4 c0 = ring.read(slot, b, 0), c1 = ring.read(slot, b, 1);
+            const unsigned word0[4] = {c0.x, c0.y, c0.z, c0.w}, word1[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                const int group = block * GROUPS + g;
-                if (group >= groups) break;                 // (behind K there are no scales)
-                const float s0 = to_f32(a.scales[row0 * a.lds + group]), s1 = to_f32(a.scales[row1 * a.lds + group]);
-                const __nv_bfloat162 z0 = bias_of(ZEROS ? a.zeros[row0 * a.lds + group] : 8u), z1 = bias_of(ZEROS ? a.zeros[row1 * a.lds + group] : 8u);
+                const float f0 = __uint_as_float((unsigned)(now[b].s0 >> (16 * g)) << 16), f1 = __uint_as_float((unsigned)(now[b].s1 >> (16 * g)) << 16);
+                const __nv_bfloat162 z0 = minus_zero_point(ZEROS ? (unsigned)(now[b].z0 >> (8 * g)) & 0xffu : 8u), z1 = minus_zero_point(ZEROS ? (unsigned)(now[b].z1 >> (8 * g)) & 0xffu : 8u);
                 float sum[MT][4] = {};
 #pragma unroll
                 for (int j = g * RUNS; j < (g + 1) * RUNS; ++j) {
-                    const int k = block * BLOCK_K + j * 32;
+                    const int k = b * BLOCK_K + j * 32;
                     unsigned v0[4], v1[4];
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) { v0[p] = two_codes(word0[j], p, z0); v1[p] = two_codes(word1[j], p, z1); }
+                    eight_codes(word0[j], z0, v0);
+                    eight_codes(word1[j], z1, v1);
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        const uint4 xv = xok[m] && k + quad * 8 < a.K ? *reinterpret_cast<const uint4*>(xr[m] + k) : zero;   // (K is a multiple of 8)
+                        uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+                        if (!LAST || t * PAIR + k + quad * 8 < a.K) xv = *reinterpret_cast<const uint4*>(xp[m] + k);      // (K is a multiple of 8)
                         mma_bf16(sum[m], v0[0], v1[0], v0[1], v1[1], xv.x, xv.y);
                         mma_bf16(sum[m], v0[2], v1[2], v0[3], v1[3], xv.z, xv.w);
                     }
@@ -114,24 +171,64 @@ __global__ void __launch_bounds__(WARPS * 32) skinny_kernel(Args a) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(i < 2 ? s0 : s1, sum[m][i], acc[m][i]);
+                    for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(i < 2 ? f0 : f1, sum[m][i], acc[m][i]);
             }
         }
+    };
+    int slot = 0;
+    for (int t = part; t < pieces; t += SHARE) {
+        bring(slot == 0 ? stream::DEPTH - 1 : slot - 1);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            now[b] = next[b];
+            next[b].fetch(a, scales0, scales1, row0, row1, (2 * (t + SHARE) + b) * GROUPS, groups);
+        }
+        stream::Ring::wait();
+        if ((t + 1) * PAIR <= a.K) multiply(slot, t, std::false_type{});
+        else multiply(slot, t, std::true_type{});
+        slot = slot + 1 == stream::DEPTH ? 0 : slot + 1;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xp[m] += SHARE * PAIR;
     }
-    // the warps' partial sums, added in a fixed order
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[warp][m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 8 * 16; i += WARPS * 32) {
-        const int tok = (i >> 4), row = n0 + (i & 15);
-        if (tok >= a.M || row >= a.N) continue;
-        float v = red[0][i >> 4][i & 15];
+        for (int i = 0; i < 4; ++i) acc[m][i] *= 64.0f;                            // (the codes were numbers of 2^-6)
+    // the sums of the warps that share a row group, added in their order
+    float (*red)[16] = reinterpret_cast<float (*)[16]>(rings);                     // [warp * 8 MT + token][row]: over the rings, which are empty now
+    if (SHARE > 1) __syncthreads();
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) v += red[w][i >> 4][i & 15];
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[warp * MT * 8 + m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
+    if (SHARE > 1) __syncthreads();
+    else __syncwarp();
+    for (int i = part * 32 + lane; i < MT * 8 * 16; i += SHARE * 32) {
+        const int tok = i >> 4, row = n0 + (i & 15);
+        if (tok >= a.M || row >= a.N) continue;
+        float v = red[tok][i & 15];
+#pragma unroll
+        for (int w = 1; w < SHARE; ++w) v += red[w * MT * 8 + tok][i & 15];
         a.out[(size_t)tok * a.ldo + row] = __float2bfloat16_rn(v);
     }
+}
+
+template <int MT, int RUNS, bool ZEROS, int SHARE, int AN_SM>
+int launch_skinny(const Args& a, cudaStream_t s) {
+    constexpr size_t smem = SHARE * stream::RING;
+    static_assert(MT * 8 * 16 * 4 <= stream::RING, "the sums lie over the rings");
+    auto kernel = skinny_kernel<MT, RUNS, ZEROS, SHARE, AN_SM>;
+    static LlmeGrants grants;
+    if (cudaError_t e = llme_grant_smem(grants, kernel, smem)) LLME_REFUSE("gemm_int4: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    llme_launch(kernel, dim3((a.N + 15) / 16), dim3(SHARE * 32), smem, s, a);
+    LLME_LAUNCH_STATUS();
+}
+template <int MT, int RUNS, bool ZEROS>
+int launch_skinny(const Args& a, cudaStream_t s) {
+    const stream::Shares by = stream::sharing((a.N + 15) / 16, (a.K + 2 * BLOCK_K - 1) / (2 * BLOCK_K), sm_count());
+    if (by.warps == 16) return launch_skinny<MT, RUNS, ZEROS, 16, 16>(a, s);
+    if (by.warps == 8) return by.an_sm == 16 ? launch_skinny<MT, RUNS, ZEROS, 8, 16>(a, s) : launch_skinny<MT, RUNS, ZEROS, 8, 24>(a, s);
+    return by.warps == 4 ? launch_skinny<MT, RUNS, ZEROS, 4, 24>(a, s) : launch_skinny<MT, RUNS, ZEROS, 2, 24>(a, s);
 }
 
 // More tokens than the weight-streaming kernel takes at once.
@@ -153,10 +250,7 @@ int launch_wide(const Args& a, cudaStream_t s) {
 template <int RUNS, bool ZEROS>
 int launch(const Args& a, cudaStream_t s) {
     if (a.M > 16) return launch_wide<RUNS, ZEROS>(a, s);
-    const int rows = (a.N + 15) / 16;
-    if (a.M <= 8) llme_launch(skinny_kernel<1, RUNS, ZEROS, 4, 8>, dim3(rows), dim3(256), 0, s, a);
-    else llme_launch(skinny_kernel<2, RUNS, ZEROS, 2, 8>, dim3(rows), dim3(256), 0, s, a);
-    LLME_LAUNCH_STATUS();
+    return a.M <= 8 ? launch_skinny<1, RUNS, ZEROS>(a, s) : launch_skinny<2, RUNS, ZEROS>(a, s);
 }
 template <int RUNS>
 int launch(const Args& a, cudaStream_t s) { return a.zeros ? launch<RUNS, true>(a, s) : launch<RUNS, false>(a, s); }
@@ -179,7 +273,9 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     const long long groups = (K + group - 1LL) / group;
     if (meets(span(out, M, N, ldo, 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
         LLME_REFUSE("gemm_int4: the output lies over an operand");
-    const Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K};
+    Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K, 0};
+    const int few = 128 / group;                            // scales of a block
+    a.vec_scales = lds % few == 0 && (uintptr_t)scales % (2 * few) == 0 && (uintptr_t)zeros % few == 0;
     if (group == 32) return launch<1>(a, stream);
     if (group == 64) return launch<2>(a, stream);
     return launch<4>(a, stream);
