@@ -106,6 +106,13 @@ class EngineConfig:
     # {"attention.portion": "mma", "linear": "cublas"} (the operations and their variants: executor.h)
     kernels: Any = "fast"
     device: str = "cuda:0"
+    # what the layers' products read: "stored": the matrices as they are; "e4m3": weights and activations of 8 bits (floating point,
+    # a scale for every row of both); "int4": weights of 4 bits with a scale for every `weight_group` values of a row (and a zero
+    # point, with `weight_zero_points`), activations in bfloat16.  Embedding and head stay as stored.  For designs made of
+    # grouped-query attention, SwiGLU and RMS norms, in bfloat16.
+    weights: str = "stored"
+    weight_group: int = 128
+    weight_zero_points: bool = False
 
     def __post_init__(self) -> None:
         if self.dtype in ("bf16",):
@@ -118,6 +125,12 @@ class EngineConfig:
             raise ConfigError(f"page_size must be in 1..256, got {self.page_size}")
         if not (self.kernels in ("fast", "plain") or isinstance(self.kernels, Mapping)):
             raise ConfigError(f"kernels must be 'fast', 'plain' or a mapping operation -> variant, got {self.kernels!r}")
+        if self.weights not in ("stored", "e4m3", "int4"):
+            raise ConfigError(f"weights must be 'stored', 'e4m3' or 'int4', got {self.weights!r}")
+        if self.weights != "stored" and self.dtype != "bfloat16":
+            raise ConfigError(f"weights {self.weights!r} need dtype bfloat16, got {self.dtype!r}")
+        if self.weight_group not in (32, 64, 128):
+            raise ConfigError(f"weight_group must be 32, 64 or 128, got {self.weight_group!r}")
         for k in ("max_num_seqs", "max_num_batched_tokens", "prefill_chunk"):
             if getattr(self, k) <= 0:
                 raise ConfigError(f"{k} must be positive")

@@ -32,6 +32,10 @@ typedef int (*EmbeddingFn)(const int*, const void*, int, float*, int, int, int, 
 typedef int (*RmsNormFn)(float*, const void*, int, const void*, int, void*, int, const int*, int, int, float, cudaStream_t);
 typedef int (*QkvPostFn)(const LlmeQkvArgs*, int, int, cudaStream_t);
 typedef int (*SwigluFn)(const void*, int, void*, int, int, int, cudaStream_t);
+typedef int (*RmsNormE4m3Fn)(const float*, const void*, int, const void*, int, float*, void*, float*, int, int, float, cudaStream_t);
+typedef int (*RowsE4m3Fn)(const void*, int, long long, void*, long long, float*, int, int, cudaStream_t);
+typedef int (*GemmE4m3Fn)(const void*, long long, const float*, const void*, long long, const float*, void*, int, long long, int, int, int, cudaStream_t);
+typedef int (*GemmInt4Fn)(const void*, long long, const void*, long long, const void*, const void*, long long, int, void*, long long, int, int, int, cudaStream_t);
 typedef int (*GemmF32Fn)(const float*, const void*, int, float*, int, int, int, long long, long long, long long, cudaStream_t);
 typedef int (*GemmBf16Fn)(const void*, long long, const void*, long long, void*, int, long long, int, int, int, cudaStream_t);
 typedef int (*GemmTcSwigluFn)(const void*, long long, const void*, long long, void*, long long, int, int, int, cudaStream_t);
@@ -211,6 +215,11 @@ size_t record_size(int kind) {
         case LLME_OP_DELTA_RULE: return sizeof(LlmeDeltaRuleOp);
         case LLME_OP_STREAM_NORM: return sizeof(LlmeStreamNormOp);
         case LLME_OP_FORGET_GATES: return sizeof(LlmeForgetGatesOp);
+        case LLME_OP_RMSNORM_E4M3: return sizeof(LlmeRmsNormE4m3Op);
+        case LLME_OP_ROWS_E4M3: return sizeof(LlmeRowsE4m3Op);
+        case LLME_OP_LINEAR_E4M3: return sizeof(LlmeLinearE4m3Op);
+        case LLME_OP_LINEAR_INT4: return sizeof(LlmeLinearInt4Op);
+        case LLME_OP_SWIGLU: return sizeof(LlmeSwigluOp);
     }
     return 0;
 }
@@ -219,8 +228,8 @@ const char* kind_name(int kind) {
                                   "linear_act", "pointwise", "batched_linear", "residual_add", "latent_attention", "token_side",
                                   "postnorm", "window_attention", "moe_route", "grouped_linear", "moe_combine", "short_conv", "rotate",
                                   "recurrence", "gated_norm", "row_norm", "exp_gates", "layernorm", "delta_rule",
-                                  "stream_norm", "forget_gates"};
-    return kind >= 1 && kind <= 29 ? names[kind] : names[0];
+                                  "stream_norm", "forget_gates", "rmsnorm_e4m3", "rows_e4m3", "linear_e4m3", "linear_int4", "swiglu"};
+    return kind >= 1 && kind <= 34 ? names[kind] : names[0];
 }
 
 constexpr int SKINNY_ROWS = 16;      // most rows the weight-streaming product takes (gemm_skinny.cu)
@@ -424,6 +433,37 @@ int op_linear_swiglu(LlmeExecutor& ex, const LlmeLinearSwigluOp& o, const LlmeSt
     if (!f) return ex.fail("no swiglu kernel is registered");
     if (o.ldo != o.inter) return ex.fail("linear_swiglu: the unfused form writes dense rows");
     return ex.launched(f(o.gate_up, o.dtype, o.out, o.dtype, M, o.inter, st), "swiglu");
+}
+
+int op_rmsnorm_e4m3(LlmeExecutor& ex, const LlmeRmsNormE4m3Op& o, const LlmeStep& s, cudaStream_t st) {
+    auto* f = (RmsNormE4m3Fn)ex.find("rmsnorm_e4m3");
+    if (!f) return ex.fail("no norm kernel that writes 8-bit rows is registered");
+    return ex.launched(f(o.x, o.delta, o.delta_dtype, o.gain, o.gain_dtype, o.x, o.out, o.scales, s.num_tokens, o.size, o.eps, st), "rmsnorm_e4m3");
+}
+
+int op_rows_e4m3(LlmeExecutor& ex, const LlmeRowsE4m3Op& o, const LlmeStep& s, cudaStream_t st) {
+    const char* name = o.gated ? "swiglu_e4m3" : "rows_e4m3";
+    auto* f = (RowsE4m3Fn)ex.find(name);
+    if (!f) return ex.fail("no kernel that writes 8-bit rows is registered");
+    return ex.launched(f(o.x, o.dtype, o.ldx, o.out, o.ldo, o.scales, s.num_tokens, o.size, st), name);
+}
+
+int op_linear_e4m3(LlmeExecutor& ex, const LlmeLinearE4m3Op& o, const LlmeStep& s, cudaStream_t st) {
+    auto* f = (GemmE4m3Fn)ex.find("gemm_e4m3");
+    if (!f) return ex.fail("no product of 8-bit rows is registered");
+    return ex.launched(f(o.x, o.ldx, o.x_scales, o.w, o.ldw, o.w_scales, o.out, o.out_dtype, o.ldo, s.num_tokens, o.n, o.k, st), "gemm_e4m3");
+}
+
+int op_linear_int4(LlmeExecutor& ex, const LlmeLinearInt4Op& o, const LlmeStep& s, cudaStream_t st) {
+    auto* f = (GemmInt4Fn)ex.find("gemm_int4");
+    if (!f) return ex.fail("no product with 4-bit weights is registered");
+    return ex.launched(f(o.x, o.ldx, o.w, o.ldw, o.scales, o.zeros, o.lds, o.group, o.out, o.ldo, s.num_tokens, o.n, o.k, st), "gemm_int4");
+}
+
+int op_swiglu(LlmeExecutor& ex, const LlmeSwigluOp& o, const LlmeStep& s, cudaStream_t st) {
+    auto* f = (SwigluFn)ex.find("swiglu");
+    if (!f) return ex.fail("no swiglu kernel is registered");
+    return ex.launched(f(o.gate_up, o.dtype, o.out, o.dtype, s.num_tokens, o.inter, st), "swiglu");
 }
 
 int op_qkv_post(LlmeExecutor& ex, const LlmeQkvPostOp& o, const LlmeStep& s, cudaStream_t st) {
@@ -1217,6 +1257,11 @@ LLME_EXPORT int llme_plan_run(LlmePlan* p, const LlmeStep* step, int first, int 
             case LLME_OP_STREAM_NORM: rc = op_stream_norm(ex, *(const LlmeStreamNormOp*)b, s, stream); break;
             case LLME_OP_FORGET_GATES: rc = op_forget_gates(ex, *(const LlmeForgetGatesOp*)b, s, stream); break;
             case LLME_OP_EXP_GATES: rc = op_exp_gates(ex, *(const LlmeExpGatesOp*)b, s, stream); break;
+            case LLME_OP_RMSNORM_E4M3: rc = op_rmsnorm_e4m3(ex, *(const LlmeRmsNormE4m3Op*)b, s, stream); break;
+            case LLME_OP_ROWS_E4M3: rc = op_rows_e4m3(ex, *(const LlmeRowsE4m3Op*)b, s, stream); break;
+            case LLME_OP_LINEAR_E4M3: rc = op_linear_e4m3(ex, *(const LlmeLinearE4m3Op*)b, s, stream); break;
+            case LLME_OP_LINEAR_INT4: rc = op_linear_int4(ex, *(const LlmeLinearInt4Op*)b, s, stream); break;
+            case LLME_OP_SWIGLU: rc = op_swiglu(ex, *(const LlmeSwigluOp*)b, s, stream); break;
             case LLME_OP_CALL: {
                 const LlmeCallOp& c = *(const LlmeCallOp*)b;
                 rc = c.fn ? c.fn(c.user, step, stream) : 0;

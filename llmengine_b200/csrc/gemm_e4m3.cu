@@ -23,6 +23,8 @@ namespace {
 
 constexpr int KC = stream::PIECE; // values (bytes) of a row in a step: two blocks of 64
 
+int g_form = 0;                   // llme_gemm_e4m3_form()
+
 struct Args {
     const unsigned char* x; long long ldx; const float* xs;
     const unsigned char* w; long long ldw; const float* ws;
@@ -144,7 +146,8 @@ int launch_wide(const Args& a, cudaStream_t s) {
     double cycles;
     if (int rc = wide::shape<false, 4, false>(g, &cycles)) return rc;
     const long long pairs = sm_count() / 2, tiles = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if ((double)((tiles + pairs - 1) / pairs) * ((a.K + 127) / 128) * 580.0 + 11000.0 < cycles) return pair::launch<O>(a, s);
+    const double paired = (double)((tiles + pairs - 1) / pairs) * ((a.K + 127) / 128) * 580.0 + 11000.0;
+    if (g_form == 2 || (g_form == 0 && paired < cycles)) return pair::launch<O>(a, s);
     alignas(64) CUtensorMap mw, mx;
     if (int rc = make_map(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, a.K, a.ldw, BM, wide::STEP)) return rc;
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, a.K, a.ldx, g.nt, wide::STEP)) return rc;
@@ -174,6 +177,13 @@ LLME_API int llme_gemm_e4m3(const void* x, long long ldx, const float* xs, const
     if (out_dtype == LLME_F32) return launch<float>(a, stream);
     if (out_dtype == LLME_BF16) return launch<bf16>(a, stream);
     LLME_REFUSE("gemm_e4m3: unsupported output dtype %d", out_dtype);
+}
+
+// More than 16 tokens: 0 (the default): whichever kernel should be faster; 1: narrow tiles, K cut over clusters; 2: pairs of SMs.  For tests
+// and measurements.
+LLME_API int llme_gemm_e4m3_form(int how) {
+    if (how >= 0 && how <= 2) g_form = how;
+    return g_form;
 }
 
 // 0 if no bounded wait has given up since the last call (synchronises the device).

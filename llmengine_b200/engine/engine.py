@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ..cache import CacheError, CacheManager, OutOfPages
-from ..config import EngineConfig, config_from_dict, load_config
+from ..config import ConfigError, EngineConfig, config_from_dict, load_config
 from ..parts.base import Runtime
 from ..weights import load_model_weights, random_model_weights
 from .batch import GroupView, StepBatch
@@ -67,8 +67,13 @@ class Engine:
         self.max_model_len = min(ec.max_model_len or self.spec.max_positions, self.spec.max_positions)
         if hasattr(ops, "choose_kernels"):
             ops.choose_kernels(ec.kernels)
-        self.rt = Runtime(ops, self.device, self.dtype, ec.max_num_batched_tokens, ec.kernels, ec.max_num_seqs)
+        self.rt = Runtime(ops, self.device, self.dtype, ec.max_num_batched_tokens, ec.kernels, ec.max_num_seqs, ec.weights, ec.weight_group,
+                          ec.weight_zero_points)
         self.model = Model(self.spec, self.rt)
+        if ec.weights != "stored":
+            other = [b.prefix for b in self.model.blocks if not b.takes_low_bit]
+            if other:
+                raise ConfigError(f"weights {ec.weights!r} are for layers of grouped-query attention, SwiGLU and RMS norms; {other[0]!r} is another kind")
         if model_dir is not None:
             load_model_weights(self.model, self.config, model_dir, self.dtype, self.device)
         else:

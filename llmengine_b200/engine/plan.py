@@ -107,6 +107,32 @@ class Plan:
         self._add("linear_swiglu", x=x, w_gate_up=w_gate_up, gate_up=gate_up, out=out, act=act,
                   params=tuple(float(p) for p in params), bias=bias)
 
+    def rmsnorm_e4m3(self, x: torch.Tensor, gain: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
+                     delta: Optional[torch.Tensor] = None) -> None:
+        """x += delta (if given), h = rmsnorm(x) * gain as rows of 8 bits: scales[t] = max(max |h_t|, 2^-100) / 448 (32-bit [T]),
+        out[t] = h_t / scales[t] (float8_e4m3fn)."""
+        self._add("rmsnorm_e4m3", x=x, gain=gain, eps=float(eps), out=out, scales=scales, delta=delta)
+        if delta is not None:
+            self.note_copy(x, None)
+
+    def rows_e4m3(self, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> None:
+        """The rows of x, or with `gated` silu(gate) * up of x = [gate | up], as rows of 8 bits (as `rmsnorm_e4m3` writes them)."""
+        self._add("rows_e4m3", x=x, out=out, scales=scales, gated=bool(gated))
+
+    def linear_e4m3(self, x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> None:
+        """out[t, n] = x_scales[t] w_scales[n] (x[t] . w[n]) for the step's tokens, x and w float8_e4m3fn."""
+        self._add("linear_e4m3", x=x, x_scales=x_scales, w=w, w_scales=w_scales, out=out)
+
+    def linear_int4(self, x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int,
+                    out: torch.Tensor) -> None:
+        """out = x w^T for the step's tokens with weights of 4 bits: w[n, k] = scales[n, k // group] (code[n, k] - zeros[n, k // group]),
+        codes as weights.quantize.pack_int4 lays them; `zeros` None: 8 everywhere."""
+        self._add("linear_int4", x=x, w=w, scales=scales, zeros=zeros, group=int(group), out=out)
+
+    def swiglu(self, gate_up: torch.Tensor, out: torch.Tensor) -> None:
+        """out = silu(gate) * up of gate_up = [gate | up]."""
+        self._add("swiglu", gate_up=gate_up, out=out)
+
     def qkv_post(self, *, q_in, k_in, v_in, num_heads: int, num_kv_heads: int, head_dim: int, q_gain=None, k_gain=None,
                  eps: float = 0.0, cos_sin=None, q_out=None, k_out=None, cache=None, group: int = 0) -> None:
         """Per-head norm (with gains), rotation (with a table) and cache write (with a cache) of what is given."""

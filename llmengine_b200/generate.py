@@ -59,6 +59,9 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--max-num-batched-tokens", type=int, default=2048)
     ap.add_argument("--prefill-chunk", type=int, default=2048)
     ap.add_argument("--kernels", choices=["fast", "plain"], default="fast")
+    ap.add_argument("--weights", choices=["stored", "e4m3", "int4"], default="stored", help="what the layers' products read: the matrices as stored, or rounded to 8 or 4 bits")
+    ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=128, help="values of a row that share a scale (--weights int4)")
+    ap.add_argument("--weight-zero-points", action="store_true", help="a zero point beside every scale (--weights int4)")
     ap.add_argument("--ignore-eos", action="store_true")
     args = ap.parse_args(argv)
 
@@ -92,7 +95,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     t0 = time.time()
     llm = LLM(args.model, dtype=args.dtype, page_size=args.page_size, max_cached_tokens=args.max_cached_tokens,
               max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
-              prefill_chunk=args.prefill_chunk, kernels=args.kernels, seed=args.seed)
+              prefill_chunk=args.prefill_chunk, kernels=args.kernels, seed=args.seed, weights=args.weights,
+              weight_group=args.weight_group, weight_zero_points=args.weight_zero_points)
     log(f"      {time.time() - t0:.1f} s")
     sp = SamplingParams(greedy=args.greedy, top_k=args.top_k, top_p=args.top_p, temperature=args.temperature,
                         repetition_penalty=args.repetition_penalty, seed=args.seed)

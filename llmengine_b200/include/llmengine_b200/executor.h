@@ -73,7 +73,8 @@ enum LlmeOpKind {
     LLME_OP_ATTENTION, LLME_OP_CALL, LLME_OP_LINEAR_ACT, LLME_OP_POINTWISE, LLME_OP_BATCHED_LINEAR, LLME_OP_RESIDUAL_ADD,
     LLME_OP_LATENT_ATTENTION, LLME_OP_TOKEN_SIDE, LLME_OP_POSTNORM, LLME_OP_WINDOW_ATTENTION, LLME_OP_MOE_ROUTE,
     LLME_OP_GROUPED_LINEAR, LLME_OP_MOE_COMBINE, LLME_OP_SHORT_CONV, LLME_OP_ROTATE, LLME_OP_RECURRENCE, LLME_OP_GATED_NORM,
-    LLME_OP_ROW_NORM, LLME_OP_EXP_GATES, LLME_OP_LAYERNORM, LLME_OP_DELTA_RULE, LLME_OP_STREAM_NORM, LLME_OP_FORGET_GATES
+    LLME_OP_ROW_NORM, LLME_OP_EXP_GATES, LLME_OP_LAYERNORM, LLME_OP_DELTA_RULE, LLME_OP_STREAM_NORM, LLME_OP_FORGET_GATES,
+    LLME_OP_RMSNORM_E4M3, LLME_OP_ROWS_E4M3, LLME_OP_LINEAR_E4M3, LLME_OP_LINEAR_INT4, LLME_OP_SWIGLU
 };
 
 enum { LLME_ACT_XIELU = 1, LLME_ACT_RELU2 = 2 };   /* 2: max(z, 0)^2 */
@@ -143,6 +144,47 @@ typedef struct LlmeLinearOp {
     int rows;                  /* LLME_ROWS_TOKENS or LLME_ROWS_LOGITS */
     const float* bias;         /* [n] added to every row of the product, or NULL */
 } LlmeLinearOp;
+
+/* Rows of 8-bit floating-point numbers (e4m3) with a 32-bit scale each (csrc/rows_e4m3.cu): h = a q, a = max(max |h|, 2^-100) / 448.
+ * x += delta (if given), h = x / sqrt(mean(x^2) + eps) * gain. */
+typedef struct LlmeRmsNormE4m3Op {
+    float* x;                  /* [T, size] the residual stream, updated in place when delta is given */
+    const void* delta; int delta_dtype;
+    const void* gain; int gain_dtype;
+    void* out; float* scales;  /* [T, size] bytes, [T] */
+    int size; float eps;
+} LlmeRmsNormE4m3Op;
+
+/* h = the rows of x [T, size], or with `gated` silu(gate) * up of x [T, 2 * size] = [gate | up]. */
+typedef struct LlmeRowsE4m3Op {
+    const void* x; long long ldx; int dtype;
+    void* out; long long ldo; float* scales;
+    int size, gated;
+} LlmeRowsE4m3Op;
+
+/* out[t, j] = x_scales[t] w_scales[j] (x[t] . w[j]), x and w e4m3 (csrc/gemm_e4m3.cu). */
+typedef struct LlmeLinearE4m3Op {
+    const void* x; long long ldx; const float* x_scales;
+    const void* w; long long ldw; const float* w_scales;
+    void* out; long long ldo; int out_dtype;
+    int n, k;
+} LlmeLinearE4m3Op;
+
+/* out = x w^T for bfloat16 x and out and 4-bit weights, w[j, i] = scales[j, i / group] (code - zeros[j, i / group]) (csrc/gemm_int4.cu);
+ * zeros NULL: 8 everywhere. */
+typedef struct LlmeLinearInt4Op {
+    const void* x; long long ldx;
+    const void* w; long long ldw;                        /* codes: bytes from row to row */
+    const void* scales; const void* zeros; long long lds; /* bfloat16, bytes */
+    void* out; long long ldo;
+    int group, n, k;
+} LlmeLinearInt4Op;
+
+/* out [T, inter] = silu(gate) * up of gate_up [T, 2 * inter], both of one type. */
+typedef struct LlmeSwigluOp {
+    const void* gate_up; void* out;
+    int dtype, inter;
+} LlmeSwigluOp;
 
 typedef struct LlmeLinearSwigluOp {
     const void* x; long long ldx; int dtype;

@@ -14,7 +14,8 @@ ROWS = {"tokens": 0, "logits": 1}
 (OP_EMBEDDING, OP_RMSNORM, OP_LINEAR, OP_LINEAR_SWIGLU, OP_QKV_POST, OP_ATTEND, OP_ATTENTION, OP_CALL, OP_LINEAR_ACT,
  OP_POINTWISE, OP_BATCHED_LINEAR, OP_RESIDUAL_ADD, OP_LATENT_ATTENTION, OP_TOKEN_SIDE, OP_POSTNORM, OP_WINDOW_ATTENTION,
  OP_MOE_ROUTE, OP_GROUPED_LINEAR, OP_MOE_COMBINE, OP_SHORT_CONV, OP_ROTATE, OP_RECURRENCE, OP_GATED_NORM, OP_ROW_NORM,
- OP_EXP_GATES, OP_LAYERNORM, OP_DELTA_RULE, OP_STREAM_NORM, OP_FORGET_GATES) = range(1, 30)
+ OP_EXP_GATES, OP_LAYERNORM, OP_DELTA_RULE, OP_STREAM_NORM, OP_FORGET_GATES, OP_RMSNORM_E4M3, OP_ROWS_E4M3, OP_LINEAR_E4M3, OP_LINEAR_INT4,
+ OP_SWIGLU) = range(1, 35)
 GATES = {"silu": 0, "clamped_swish": 1, "gelu_tanh": 2}
 ROUTING = {"sigmoid": 0, "softmax_chosen": 1, "softmax": 2}
 ACTIVATIONS = {"xielu": 1, "relu2": 2}
@@ -63,6 +64,30 @@ class StreamNormOp(Structure):
     _fields_ = [("x", c_void_p), ("streams", c_int), ("size", c_int), ("y", c_void_p), ("gate", c_void_p), ("ldg", c_longlong),
                 ("gate_dtype", c_int), ("gate_bias", c_void_p), ("mix", c_void_p), ("put", c_void_p), ("read", c_void_p), ("gain", c_void_p),
                 ("eps", c_float), ("out", c_void_p), ("out_dtype", c_int), ("rows", c_int)]
+
+
+class RmsNormE4m3Op(Structure):
+    _fields_ = [("x", c_void_p), ("delta", c_void_p), ("delta_dtype", c_int), ("gain", c_void_p), ("gain_dtype", c_int), ("out", c_void_p),
+                ("scales", c_void_p), ("size", c_int), ("eps", c_float)]
+
+
+class RowsE4m3Op(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_longlong), ("dtype", c_int), ("out", c_void_p), ("ldo", c_longlong), ("scales", c_void_p),
+                ("size", c_int), ("gated", c_int)]
+
+
+class LinearE4m3Op(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_longlong), ("x_scales", c_void_p), ("w", c_void_p), ("ldw", c_longlong), ("w_scales", c_void_p),
+                ("out", c_void_p), ("ldo", c_longlong), ("out_dtype", c_int), ("n", c_int), ("k", c_int)]
+
+
+class LinearInt4Op(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_longlong), ("w", c_void_p), ("ldw", c_longlong), ("scales", c_void_p), ("zeros", c_void_p),
+                ("lds", c_longlong), ("out", c_void_p), ("ldo", c_longlong), ("group", c_int), ("n", c_int), ("k", c_int)]
+
+
+class SwigluOp(Structure):
+    _fields_ = [("gate_up", c_void_p), ("out", c_void_p), ("dtype", c_int), ("inter", c_int)]
 
 
 class ForgetGatesOp(Structure):
@@ -300,6 +325,11 @@ def _attend_record(a: Dict[str, Any]) -> AttendOp:
                     scratch.numel() if scratch is not None else 0)
 
 
+def _rows8(q: torch.Tensor, scales: torch.Tensor) -> bool:
+    return (q.dtype == torch.float8_e4m3fn and q.stride(1) == 1 and scales.dtype == torch.float32 and scales.is_contiguous()
+            and scales.numel() == q.shape[0])
+
+
 def records(op, keep: List[Any]):
     """(kind, ctypes record) of one plan operation; `keep` collects what must stay alive with the plan."""
     a = op.a
@@ -337,6 +367,35 @@ def records(op, keep: List[Any]):
         return OP_LINEAR, LinearOp(x.data_ptr(), x.stride(0), code(x.dtype), w.data_ptr(), w.stride(0), code(w.dtype), ptr(out),
                                    out.stride(0) if out is not None else 0, code(out.dtype) if out is not None else F32,
                                    w.shape[0], w.shape[1], ROWS[a["rows"]], ptr(a.get("bias")))
+    if k == "rmsnorm_e4m3":
+        x, d, g, out, sc = a["x"], a["delta"], a["gain"], a["out"], a["scales"]
+        assert x.dtype == torch.float32 and x.is_contiguous() and (d is None or (d.is_contiguous() and d.shape == x.shape))
+        assert g.is_contiguous() and g.numel() == x.shape[1] and _rows8(out, sc) and out.is_contiguous() and out.shape[1] == x.shape[1]
+        return OP_RMSNORM_E4M3, RmsNormE4m3Op(x.data_ptr(), ptr(d), code(d.dtype) if d is not None else 0, g.data_ptr(), code(g.dtype),
+                                              out.data_ptr(), sc.data_ptr(), x.shape[1], a["eps"])
+    if k == "rows_e4m3":
+        x, out, sc, gated = a["x"], a["out"], a["scales"], bool(a["gated"])
+        assert x.stride(1) == 1 and _rows8(out, sc) and x.shape[1] == (2 if gated else 1) * out.shape[1]
+        return OP_ROWS_E4M3, RowsE4m3Op(x.data_ptr(), x.stride(0), code(x.dtype), out.data_ptr(), out.stride(0), sc.data_ptr(), out.shape[1],
+                                        int(gated))
+    if k == "linear_e4m3":
+        x, xs, w, ws, out = a["x"], a["x_scales"], a["w"], a["w_scales"], a["out"]
+        assert _rows8(x, xs) and _rows8(w, ws) and w.shape[1] == x.shape[1] and out.stride(1) == 1 and out.shape[1] == w.shape[0]
+        return OP_LINEAR_E4M3, LinearE4m3Op(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(), out.data_ptr(),
+                                            out.stride(0), code(out.dtype), w.shape[0], w.shape[1])
+    if k == "linear_int4":
+        x, w, sc, z, out = a["x"], a["w"], a["scales"], a["zeros"], a["out"]
+        assert x.dtype == out.dtype == torch.bfloat16 and x.stride(1) == 1 and out.stride(1) == 1 and out.shape[1] == w.shape[0]
+        assert w.dtype == torch.uint8 and w.stride(1) == 1 and w.shape[1] == -(-x.shape[1] // 128) * 64
+        groups = (w.shape[0], -(-x.shape[1] // a["group"]))
+        assert sc.dtype == torch.bfloat16 and sc.is_contiguous() and sc.shape == groups
+        assert z is None or (z.dtype == torch.uint8 and z.is_contiguous() and z.shape == groups)
+        return OP_LINEAR_INT4, LinearInt4Op(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), sc.data_ptr(), ptr(z), groups[1],
+                                            out.data_ptr(), out.stride(0), a["group"], w.shape[0], x.shape[1])
+    if k == "swiglu":
+        gu, out = a["gate_up"], a["out"]
+        assert gu.is_contiguous() and out.is_contiguous() and gu.dtype == out.dtype and gu.shape[1] == 2 * out.shape[1]
+        return OP_SWIGLU, SwigluOp(gu.data_ptr(), out.data_ptr(), code(out.dtype), out.shape[1])
     if k == "linear_swiglu":
         x, w, gu, out = a["x"], a["w_gate_up"], a["gate_up"], a["out"]
         assert x.dtype == w.dtype == out.dtype and x.stride(1) == 1 and w.stride(1) == 1 and out.stride(1) == 1

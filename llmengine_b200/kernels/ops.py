@@ -223,6 +223,9 @@ class CudaOps:
                         "gemm_skinny_act": "llme_gemm_skinny_act_bf16", "gemm_skinny_gated": "llme_gemm_skinny_gated_bf16"},
         "gemm_tcgen05": {"gemm_tc": "llme_gemm_tc_bf16", "gemm_tc_swiglu": "llme_gemm_tc_swiglu_bf16",
                          "gemm_tc_act": "llme_gemm_tc_act_bf16", "gemm_tc_gated": "llme_gemm_tc_gated_bf16"},
+        "rows_e4m3": {"rmsnorm_e4m3": "llme_rmsnorm_e4m3", "rows_e4m3": "llme_rows_e4m3", "swiglu_e4m3": "llme_swiglu_e4m3"},
+        "gemm_e4m3": {"gemm_e4m3": "llme_gemm_e4m3"},
+        "gemm_int4": {"gemm_int4": "llme_gemm_int4"},
         "attention_plain": {"attention_plain": "llme_attention_plain"},
         "attention_fast": {"attention_portion/{hd}": "llme_attention_portion", "attention_decode/{hd}": "llme_attention_decode",
                            "attention_decode_fused/{hd}": "llme_attention_decode_fused",
@@ -259,6 +262,14 @@ class CudaOps:
                 want("pointwise")
             if op.kind == "stream_norm":
                 want("streams")
+            if op.kind in ("rmsnorm_e4m3", "rows_e4m3"):
+                want("rows_e4m3")
+            if op.kind == "linear_e4m3":
+                want("gemm_e4m3")
+            if op.kind == "linear_int4":
+                want("gemm_int4")
+            if op.kind == "swiglu":
+                want("elementwise")
             if op.kind == "linear_swiglu" and (a.get("act", "silu") != "silu" or a.get("bias") is not None):
                 want("pointwise")
             if op.kind == "linear" and a.get("bias") is not None:
@@ -665,6 +676,11 @@ class CudaOps:
             self._launch("gemm_e4m3", what, fn, x.data_ptr(), self._row_stride(x), x_scales.data_ptr(), w.data_ptr(), self._row_stride(w),
                          w_scales.data_ptr(), out.data_ptr(), _code(out.dtype), self._row_stride(out), M, N, K)
         return out
+
+    def linear_e4m3_form(self, how: str) -> None:
+        """Which kernel multiplies more than 16 rows by 8-bit weights: "auto" (the one that should be faster), "wide" (narrow tiles, K cut
+        over clusters) or "pair" (256 x 256 tiles on pairs of SMs).  For tests and measurements."""
+        self._lib("gemm_e4m3").llme_gemm_e4m3_form(c_int({"auto": 0, "wide": 1, "pair": 2}[how]))
 
     @staticmethod
     def int4_group(k: int, groups: int) -> int:

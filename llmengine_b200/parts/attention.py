@@ -11,6 +11,7 @@ from ..config.spec import PartSpec
 from ..engine.plan import Plan
 from dataclasses import dataclass
 
+from .low_bit import emit_linear, hold, result_dtype
 from .base import (PagedAndStateSpec, PagedAndStateView, PagedKVSpec, Part, Runtime, StatesSpec, WeightSpec, build_part,
                    register_part, run_alone)
 
@@ -29,6 +30,8 @@ class GQAttention(Part):
 
     The three projections are stored as one matrix [q | k | v] so that one product serves them.
     """
+
+    takes_low_bit = True
 
     def __init__(self, rt: Runtime, prefix: str, hidden_size: int, num_heads: int, num_kv_heads: int,
                  head_dim: int, qk_norm_eps: Optional[float], position_encoding: PartSpec, window: int = 0):
@@ -57,9 +60,9 @@ class GQAttention(Part):
         return s
 
     def load_weights(self, t: Dict[str, torch.Tensor]) -> None:
-        self.w_qkv = torch.cat([t[self.name("q_proj.weight")], t[self.name("k_proj.weight")],
-                                t[self.name("v_proj.weight")]], dim=0).contiguous()
-        self.w_o = t[self.name("o_proj.weight")].contiguous()
+        self.w_qkv = hold(self.rt, torch.cat([t[self.name("q_proj.weight")], t[self.name("k_proj.weight")],
+                                              t[self.name("v_proj.weight")]], dim=0).contiguous(), f"{self.prefix} q, k, v")
+        self.w_o = hold(self.rt, t[self.name("o_proj.weight")].contiguous(), self.name("o_proj.weight"))
         if self.eps is not None:
             qg, kg = t[self.name("q_norm.weight")], t[self.name("k_norm.weight")]
             if qg.dtype != kg.dtype:          # one kernel launch takes one gain type
@@ -79,7 +82,7 @@ class GQAttention(Part):
         writes = cache.writes
         width = qs + 2 * kvs if writes else qs
         qkv = rt.workspace("qkv", width, rt.dtype)
-        plan.linear(h, self.w_qkv[:width], qkv)
+        emit_linear(plan, rt, h, self.w_qkv[:width], qkv, "normed_rows8")
         q = rt.workspace("q", qs, rt.dtype)
         out = rt.workspace("attn_out", qs, rt.dtype)
         scratch = rt.attention_scratch(self.nh, self.nkv, self.hd)
@@ -99,8 +102,8 @@ class GQAttention(Part):
             if writes:
                 plan.qkv_post(q_in=None, k_in=k, v_in=qkv[:, qs + kvs:], **common)
             plan.attend(q=q, out=out, window=self.window, scale=self.scale, scratch=scratch, **common)
-        delta = rt.workspace("mixer_out", self.hidden, torch.float32)
-        plan.linear(out, self.w_o, delta)
+        delta = rt.workspace("mixer_out", self.hidden, result_dtype(rt))
+        emit_linear(plan, rt, out, self.w_o, delta, "attn_rows8")
         return delta
 
     def forward(self, h: torch.Tensor, batch, cache) -> torch.Tensor:

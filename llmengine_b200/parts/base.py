@@ -207,6 +207,8 @@ class Part:
     # True for a part whose first product of its input can carry further rows for someone else who multiplies the same input
     # (`carry_rows`)
     carries_rows = False
+    # True for a part that also works with weights of 8 or 4 bits (parts/low_bit.py)
+    takes_low_bit = False
 
     def __init__(self, rt: "Runtime", prefix: str):
         self.rt = rt
@@ -258,13 +260,15 @@ class Runtime:
     workspace of reusable buffers."""
 
     def __init__(self, ops: Any, device: torch.device, dtype: torch.dtype, max_tokens: int, kernels: Any = "fast",
-                 max_requests: int = 64):
+                 max_requests: int = 64, weights: str = "stored", weight_group: int = 128, weight_zero_points: bool = False):
         self.ops = ops
         self.device = device
         self.dtype = dtype                 # type of matrix-product operands: bfloat16 or float32
         self.max_tokens = max_tokens
         self.max_requests = max_requests   # most requests in one step
         self.kernels = kernels
+        self.weights = weights             # what the layers' products read: "stored", "e4m3" or "int4"
+        self.weight_group, self.weight_zero_points = weight_group, weight_zero_points
         self._buffers: Dict[Tuple[str, torch.dtype], torch.Tensor] = {}
         self._views: Dict[Tuple[str, torch.dtype, int, int], torch.Tensor] = {}   # the views handed out, by shape
         self._tables: Dict[Any, torch.Tensor] = {}

@@ -51,16 +51,26 @@ class PreNormResidualBlock(Part):
         for p in self.parts:
             p.load_weights({n: tensors[n] for n in p.weight_specs()})
 
+    @property
+    def takes_low_bit(self) -> bool:
+        return all(p.takes_low_bit for p in self.parts)
+
     def cache_spec(self):
         return self.mixer.cache_spec()
 
+    def _normed(self, plan: Plan, norm: Part, x: torch.Tensor, delta: Optional[torch.Tensor]):
+        """The norm's output as the sublayer behind it takes it: in 8 bits where its weights are."""
+        if self.rt.weights == "e4m3":
+            return norm.emit_rows8(plan, x, delta=delta)
+        return emit_norm(plan, norm, x, delta=delta)
+
     def emit(self, plan: Plan, x: torch.Tensor, delta: Optional[torch.Tensor], cache) -> Tuple[torch.Tensor, torch.Tensor]:
         hidden = x.shape[1]
-        h = emit_norm(plan, self.mixer_norm, x, delta=delta)
+        h = self._normed(plan, self.mixer_norm, x, delta)
         a = emit_mixer(plan, self.mixer, h, cache, hidden)
         if self.ffn is None:
             return x, a
-        h = emit_norm(plan, self.ffn_norm, x, delta=a)
+        h = self._normed(plan, self.ffn_norm, x, a)
         return x, emit_feed_forward(plan, self.ffn, h, hidden)
 
     def forward(self, x: torch.Tensor, delta: Optional[torch.Tensor], batch, cache) -> Tuple[torch.Tensor, torch.Tensor]:

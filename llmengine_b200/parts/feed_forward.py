@@ -7,6 +7,7 @@ import torch
 
 from ..engine.plan import Plan
 from .base import Part, Runtime, WeightSpec, register_part, run_alone
+from .low_bit import emit_linear, hold, result_dtype, rows8_place
 
 
 @register_part("feed_forward", "swiglu")
@@ -15,6 +16,8 @@ class SwiGLU(Part):
     (src/model/transformer_graph_builder.cpp:261-274; src/runtime/kernels/cpu_kernels.cpp:848-859).
     The gate and up matrices are stored as one [gate | up] matrix so that one product serves both; where a
     kernel carries the activation in its epilogue the [T, 2 * intermediate] product never exists in memory."""
+
+    takes_low_bit = True
 
     def __init__(self, rt: Runtime, prefix: str, hidden_size: int, intermediate_size: int):
         super().__init__(rt, prefix)
@@ -29,16 +32,25 @@ class SwiGLU(Part):
         }
 
     def load_weights(self, t: Dict[str, torch.Tensor]) -> None:
-        self.w_gate_up = torch.cat([t[self.name("gate_proj.weight")], t[self.name("up_proj.weight")]], 0).contiguous()
-        self.w_down = t[self.name("down_proj.weight")].contiguous()
+        self.w_gate_up = hold(self.rt, torch.cat([t[self.name("gate_proj.weight")], t[self.name("up_proj.weight")]], 0).contiguous(), f"{self.prefix} gate, up")
+        self.w_down = hold(self.rt, t[self.name("down_proj.weight")].contiguous(), self.name("down_proj.weight"))
 
     def emit(self, plan: Plan, h: torch.Tensor) -> torch.Tensor:
         rt = self.rt
-        act = rt.workspace("act", self.inter, rt.dtype)
         gate_up = rt.workspace("gate_up", 2 * self.inter, rt.dtype)
-        plan.linear_swiglu(h, self.w_gate_up, gate_up, act)
-        delta = rt.workspace("ffn_out", self.hidden, torch.float32)
-        plan.linear(act, self.w_down, delta)
+        delta = rt.workspace("ffn_out", self.hidden, result_dtype(rt))
+        if rt.weights == "e4m3":
+            emit_linear(plan, rt, h, self.w_gate_up, gate_up, "normed_rows8")
+            act = rows8_place(rt, "act_rows8", self.inter)
+            plan.rows_e4m3(gate_up, act.data, act.scales, gated=True)
+        else:
+            act = rt.workspace("act", self.inter, rt.dtype)
+            if rt.weights == "stored":
+                plan.linear_swiglu(h, self.w_gate_up, gate_up, act)
+            else:
+                emit_linear(plan, rt, h, self.w_gate_up, gate_up, "normed_rows8")
+                plan.swiglu(gate_up, act)
+        emit_linear(plan, rt, act, self.w_down, delta, "act_rows8")
         return delta
 
     def forward(self, h: torch.Tensor, batch=None) -> torch.Tensor:

@@ -7,6 +7,7 @@ import torch
 
 from ..engine.plan import ROWS_LOGITS, ROWS_TOKENS, Plan, StreamUpdate
 from .base import Part, Runtime, WeightSpec, register_part, run_alone
+from .low_bit import Rows8, rows8_place
 
 
 @register_part("norm", "rmsnorm")
@@ -15,6 +16,8 @@ class RMSNorm(Part):
     (src/runtime/kernels/cpu_kernels.cpp:225-256).  The reference adds the residual with a
     separate Add node before the norm (src/model/transformer_graph_builder.cpp:251-257); here
     the norm kernel takes the not-yet-added contribution `delta` and does both."""
+
+    takes_low_bit = True
 
     def __init__(self, rt: Runtime, prefix: str, size: int, eps: float, leaf: str = "weight"):
         super().__init__(rt, prefix)
@@ -33,6 +36,12 @@ class RMSNorm(Part):
              out_name: Optional[str] = None) -> torch.Tensor:
         out = self.rt.workspace(out_name or ("normed" if rows == ROWS_TOKENS else "normed_rows"), self.size, self.rt.dtype)
         plan.rmsnorm(x, self.gain, self.eps, out, delta=delta, rows=rows)
+        return out
+
+    def emit_rows8(self, plan: Plan, x: torch.Tensor, delta: Optional[torch.Tensor] = None) -> Rows8:
+        """The normed rows in 8 bits, for products with 8-bit weights."""
+        out = rows8_place(self.rt, "normed_rows8", self.size)
+        plan.rmsnorm_e4m3(x, self.gain, self.eps, out.data, out.scales, delta=delta)
         return out
 
     def pairs_with(self, other) -> bool:

@@ -52,18 +52,26 @@ def _exact_e4m3(x, xs, w, ws):
     return (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
 
 
+@pytest.fixture(params=["wide", "pair", "auto"])
+def e4m3(ops, request):
+    """The product of 8-bit rows also by the kernel that its own choice would not take."""
+    ops.linear_e4m3_form(request.param)
+    yield ops
+    ops.linear_e4m3_form("auto")
+
+
 M_SIZES = [1, 2, 8, 9, 16, 17, 24, 33, 64, 77, 128, 129, 200, 256, 257, 513]
 
 
 @pytest.mark.parametrize("m", M_SIZES)
 @pytest.mark.parametrize("n,k", [(1, 16), (8, 128), (100, 144), (129, 4096), (1000, 272), (2048, 1040), (264, 12288)])
-def test_e4m3_places(ops, m, n, k):
+def test_e4m3_places(e4m3, m, n, k):
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=m + n + k)
     want = _exact_e4m3(x, xs, w, ws)
     for dtype in (torch.float32, torch.bfloat16):
         for extra in (0, 5):
             whole, out = _out(m, n, dtype, extra)
-            assert ops.linear_e4m3(x, xs, w, ws, out) is out
+            assert e4m3.linear_e4m3(x, xs, w, ws, out) is out
             assert torch.equal(out.double(), want.to(dtype).double())
             _rest_untouched(whole, n)
 
@@ -71,19 +79,19 @@ def test_e4m3_places(ops, m, n, k):
 @pytest.mark.parametrize("m", [1, 8, 16, 40, 77, 128, 300, 1024])
 @pytest.mark.parametrize("n,k", [(512, 4096), (264, 12288), (4096, 528)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_e4m3_rounding(ops, m, n, k, dtype):
+def test_e4m3_rounding(e4m3, m, n, k, dtype):
     from llmengine_b200.weights.quantize import quantize_e4m3
     g = _gen(m + n)
     x, xs = quantize_e4m3((torch.randn(m, k, generator=g) * 3).to(DEV))
     w, ws = quantize_e4m3((torch.randn(n, k, generator=g) * 0.02).to(DEV))
     _, out = _out(m, n, dtype)
-    ops.linear_e4m3(x, xs, w, ws, out)
+    e4m3.linear_e4m3(x, xs, w, ws, out)
     want, size = _exact_e4m3(x, xs, w, ws), _exact_e4m3(x.float().abs(), xs, w.float().abs(), ws)
     assert torch.all((out.double() - want).abs() <= _bound(dtype, want, size, k))
 
 
 @pytest.mark.parametrize("m", [3, 16, 40, 130, 300])
-def test_e4m3_strides(ops, m):
+def test_e4m3_strides(e4m3, m):
     """Operands that are columns and rows of larger matrices."""
     n, k = 200, 400
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=m)
@@ -94,13 +102,13 @@ def test_e4m3_strides(ops, m):
     big_w.view(torch.uint8)[:2] = 0x7F
     big_w.view(torch.uint8)[2 + n:] = 0x7F
     whole, out = _out(m, n, torch.bfloat16, 8)
-    ops.linear_e4m3(big_x[:, 32:32 + k], xs, big_w[2:2 + n, :k], ws, out)
+    e4m3.linear_e4m3(big_x[:, 32:32 + k], xs, big_w[2:2 + n, :k], ws, out)
     assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws).to(torch.bfloat16).double())
     _rest_untouched(whole, n)
 
 
 @pytest.mark.parametrize("m", [4, 16, 40, 200, 300])
-def test_e4m3_rows_that_are_no_numbers(ops, m):
+def test_e4m3_rows_that_are_no_numbers(e4m3, m):
     n, k = 300, 512
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=1)
     clean = _exact_e4m3(x, xs, w, ws)
@@ -109,7 +117,7 @@ def test_e4m3_rows_that_are_no_numbers(ops, m):
     x.view(torch.uint8)[2, 5] = 0x7F
     w.view(torch.uint8)[250, 3] = 0xFF
     _, out = _out(m, n, torch.float32)
-    ops.linear_e4m3(x, xs, w, ws, out)
+    e4m3.linear_e4m3(x, xs, w, ws, out)
     bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
     bad[1:3] = True
     bad[:, 250] = True

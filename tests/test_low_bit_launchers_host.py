@@ -88,3 +88,33 @@ def test_products_of_4_bits(compiled):  # noqa: F811
     assert call(lib, "llme_gemm_int4", INT4_TYPES, INT4, zeros=None) == (0, 1)
     for changed in (dict(M=0), dict(N=0)):
         assert call(lib, "llme_gemm_int4", INT4_TYPES, INT4, **changed) == (0, 0)
+
+
+@pytest.mark.parametrize("key,name", [("gemm_e4m3", "llme_gemm_e4m3_status"), ("gemm_int4", "llme_gemm_int4_status")])
+def test_a_wait_that_gave_up_is_told_once(compiled, key, name):  # noqa: F811
+    lib = compiled(key)
+    status = getattr(lib, name)
+    assert status() == 0
+    lib.fake_flag(0, 5, 0)                                 # by a kernel that still runs: the device is waited for
+    assert status() == 5 and status() == 0
+    lib.fake_flag(0, 0, 1)
+    assert status() == -1
+    lib.fake_flag(0, 0, 0)
+    from llmengine_b200.engine.engine import Engine
+    assert Engine._STATUS[key] == name
+
+
+def test_every_size_is_launched_on_every_device(compiled):  # noqa: F811
+    """The forms for few, more and many rows ask for their shared memory on the device they are launched on."""
+    e4m3, int4 = compiled("gemm_e4m3"), compiled("gemm_int4")
+    for device in (0, 1, 65):
+        e4m3.fake_device(device), int4.fake_device(device)
+        for n in (16, 2048, 4096, 6144, 12288, 24576):
+            for m in (1, 16, 17, 77, 300, 4096):
+                for k in (128, 4096):
+                    for dtype in (0, 1):
+                        assert call(e4m3, "llme_gemm_e4m3", E4M3_TYPES, E4M3, M=m, N=n, K=k, ldx=k, ldw=k, ldo=n, out_dtype=dtype, w=p(64), out=p(128)) == (0, 1)
+                    for group in (32, 64, 128):
+                        assert call(int4, "llme_gemm_int4", INT4_TYPES, INT4, M=m, N=n, K=k, ldx=k, ldw=k // 2, lds=k // group, group=group, ldo=n, w=p(64), scales=p(90),
+                                    zeros=p(100) if group == 32 else None, out=p(128)) == (0, 1)
+    e4m3.fake_device(0), int4.fake_device(0)
