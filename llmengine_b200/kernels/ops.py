@@ -35,8 +35,10 @@ class KernelError(RuntimeError):
 
 
 _F32, _BF16 = 0, 1
-_FLOAT, _FLOATS, _BF16S, _E4M3, _BYTES = (torch.float32,), (torch.float32, torch.bfloat16), (torch.bfloat16,), (torch.float8_e4m3fn,), (torch.uint8,)
+_F32T, _BF16T, _F8, _BYTE = torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8
+_FLOAT, _FLOATS, _BF16S, _E4M3, _BYTES = (_F32T,), (_F32T, _BF16T), (_BF16T,), (_F8,), (_BYTE,)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _code(dt: torch.dtype) -> int:
@@ -382,7 +384,8 @@ class CudaOps:
         return c_void_p(torch.cuda.current_stream().cuda_stream)
 
     # ------------------------------------------------------------------ operands of the methods that check what they are given
-    # (Each check asks the usual case first: a call of a few microseconds on the GPU should not take many times that here.)
+    # (A call of a few microseconds on the GPU should not take many times that here.  So each method first asks in one breath whether all
+    # operands are of the usual kind, dense and on this device; only where they are not does `_operand` say which one is at fault, or that none is.)
     def _operand(self, what: str, name: str, t: torch.Tensor, dtypes, shape=None, dense: bool = False) -> torch.Tensor:
         """`t` is a tensor on this device of one of the types and of the shape (None: any matrix), its last dimension without gaps,
         with `dense` none at all."""
@@ -404,20 +407,18 @@ class CudaOps:
 
     def _entry(self, key: str, entry: str, *types):
         """A library's entry point with its argument types; the last argument is the stream."""
-        fn = self._typed.get(entry)
-        if fn is None:
-            fn = getattr(self._lib(key), entry)
-            fn.argtypes = [*types, c_void_p]
-            self._typed[entry] = fn
+        fn = getattr(self._lib(key), entry)
+        fn.argtypes = [*types, c_void_p]
+        self._typed[entry] = fn
         return fn
 
     def _launch(self, key: str, what: str, fn, *args) -> None:
         """An entry point on torch's current stream of this device, with this device the current one."""
-        if torch.cuda.current_device() == self._device_index:
-            rc = fn(*args, self._stream())
+        if _current_device() == self._device_index:
+            rc = fn(*args, _raw_stream(self._device_index))
         else:
             with torch.cuda.device(self._device_index):
-                rc = fn(*args, self._stream())
+                rc = fn(*args, _raw_stream(self._device_index))
         if rc != 0:
             raise KernelError(f"{what}: {self._libs[key].llme_last_error().decode('utf-8', 'replace')} (code {rc})")
         self._direct += 1
@@ -596,10 +597,25 @@ class CudaOps:
         return out
 
     # ------------------------------------------------------------------ rows of 8-bit numbers
-    def _quantised_places(self, what: str, rows: int, size: int, out: torch.Tensor, scales: torch.Tensor) -> None:
+    def _rows_of(self, what: str, name: str, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, halves: int):
+        """(rows, values of an output row, row stride of x, row stride of out) for 8-bit rows of x, `halves` of its columns an output value."""
+        d = self._device_index
+        if (x.get_device() == d == out.get_device() and scales.get_device() == d and x.dtype in _FLOATS and out.dtype is _F8 and scales.dtype is _F32T
+                and x.dim() == 2 and x.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
+            rows, cols = x.shape
+            size = cols // halves
+            if out.shape == (rows, size) and scales.shape == (rows,) and cols and size * halves == cols:
+                return rows, size, cols, size
+        rows, cols = self._operand(what, name, x, _FLOATS).shape
+        if cols % halves:
+            raise KernelError(f"{what}: {name} must have an even number of columns, got {cols}")
+        self._places8(what, rows, cols // halves, out, scales)
+        return rows, cols // halves, self._row_stride(x), self._row_stride(out)
+
+    def _places8(self, what: str, rows: int, size: int, out: torch.Tensor, scales: torch.Tensor, dense: bool = False) -> None:
         if rows and not size:
             raise KernelError(f"{what}: the rows have no values")
-        self._operand(what, "out", out, _E4M3, (rows, size))
+        self._operand(what, "out", out, _E4M3, (rows, size), dense)
         self._operand(what, "scales", scales, _FLOAT, (rows,), dense=True)
 
     def rmsnorm_e4m3(self, x: torch.Tensor, gain: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
@@ -610,21 +626,25 @@ class CudaOps:
         Returns (out, scales)."""
         what = "rmsnorm_e4m3"
         rows, size = self._operand(what, "x", x, _FLOAT, dense=True).shape
-        self._operand(what, "gain", gain, _FLOATS, (size,), dense=True)
+        d, shape = self._device_index, x.shape
+        if not (gain.get_device() == d == out.get_device() and scales.get_device() == d and gain.dtype in _FLOATS and out.dtype is _F8
+                and scales.dtype is _F32T and gain.shape == (size,) and out.shape == shape and scales.shape == (rows,) and size
+                and gain.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
+            self._operand(what, "gain", gain, _FLOATS, (size,), dense=True)
+            self._places8(what, rows, size, out, scales, dense=True)
         if not eps > 0.0:
             raise KernelError(f"{what}: eps must be positive, got {eps}")
         if delta is not None:
-            self._operand(what, "delta", delta, _FLOATS, (rows, size), dense=True)
+            self._operand(what, "delta", delta, _FLOATS, shape, dense=True)
             if total is None:
                 total = x
             elif total is not x:
-                self._operand(what, "total", total, _FLOAT, (rows, size), dense=True)
+                self._operand(what, "total", total, _FLOAT, shape, dense=True)
         elif total is not None:
             raise KernelError(f"{what}: without a delta there is no sum to write")
-        self._operand(what, "out", out, _E4M3, (rows, size), dense=True)
-        self._quantised_places(what, rows, size, out, scales)
         if rows:
-            fn = self._entry("rows_e4m3", "llme_rmsnorm_e4m3", c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float)
+            fn = self._typed.get("llme_rmsnorm_e4m3") or self._entry("rows_e4m3", "llme_rmsnorm_e4m3", c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                                                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_float)
             self._launch("rows_e4m3", what, fn, x.data_ptr(), _ptr(delta), _code(delta.dtype) if delta is not None else 0, gain.data_ptr(),
                          _code(gain.dtype), _ptr(total), out.data_ptr(), scales.data_ptr(), rows, size, eps)
         return out, scales
@@ -632,47 +652,43 @@ class CudaOps:
     def rows_e4m3(self, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
         """The rows of x [T, D] (32-bit or bfloat16, any row stride) as 8-bit rows: scales[i] = max(max |x_i|, 2^-100) / 448,
         out[i] = x_i / scales[i] in float8_e4m3fn (any row stride).  Returns (out, scales)."""
-        what = "rows_e4m3"
-        rows, size = self._operand(what, "x", x, _FLOATS).shape
-        self._quantised_places(what, rows, size, out, scales)
+        rows, size, ldx, ldo = self._rows_of("rows_e4m3", "x", x, out, scales, 1)
         if rows:
-            fn = self._entry("rows_e4m3", "llme_rows_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int)
-            self._launch("rows_e4m3", what, fn, x.data_ptr(), _code(x.dtype), self._row_stride(x), out.data_ptr(), self._row_stride(out),
-                         scales.data_ptr(), rows, size)
+            fn = self._typed.get("llme_rows_e4m3") or self._entry("rows_e4m3", "llme_rows_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong,
+                                                                  c_void_p, c_int, c_int)
+            self._launch("rows_e4m3", "rows_e4m3", fn, x.data_ptr(), _code(x.dtype), ldx, out.data_ptr(), ldo, scales.data_ptr(), rows, size)
         return out, scales
 
     def swiglu_e4m3(self, gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor):
         """silu(gate) * up of gate_up [T, 2 D] = [gate | up] (32-bit or bfloat16, any row stride) as 8-bit rows, as `rows_e4m3` makes
         them.  Returns (out, scales)."""
-        what = "swiglu_e4m3"
-        rows, both = self._operand(what, "gate_up", gate_up, _FLOATS).shape
-        if both % 2:
-            raise KernelError(f"{what}: gate_up must have an even number of columns, got {both}")
-        self._quantised_places(what, rows, both // 2, out, scales)
+        rows, size, ldx, ldo = self._rows_of("swiglu_e4m3", "gate_up", gate_up, out, scales, 2)
         if rows:
-            fn = self._entry("rows_e4m3", "llme_swiglu_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int)
-            self._launch("rows_e4m3", what, fn, gate_up.data_ptr(), _code(gate_up.dtype), self._row_stride(gate_up), out.data_ptr(),
-                         self._row_stride(out), scales.data_ptr(), rows, both // 2)
+            fn = self._typed.get("llme_swiglu_e4m3") or self._entry("rows_e4m3", "llme_swiglu_e4m3", c_void_p, c_int, c_longlong, c_void_p, c_longlong,
+                                                                    c_void_p, c_int, c_int)
+            self._launch("rows_e4m3", "swiglu_e4m3", fn, gate_up.data_ptr(), _code(gate_up.dtype), ldx, out.data_ptr(), ldo, scales.data_ptr(), rows, size)
         return out, scales
 
     # ------------------------------------------------------------------ products with weights of 8 and 4 bits
-    def _product_places(self, what: str, x: torch.Tensor, n: int, out: torch.Tensor, dtypes) -> None:
-        rows = x.shape[0]
-        self._operand(what, "out", out, dtypes, (rows, n))
-
     def linear_e4m3(self, x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """out[m, n] = x_scales[m] w_scales[n] (x[m] . w[n]) for x [M, K] and w [N, K] in float8_e4m3fn, scales 32-bit, out [M, N] 32-bit
         or bfloat16; sums are 32-bit.  K is a multiple of 16, the rows of x and w begin on 16 bytes (any such row stride)."""
-        what = "linear_e4m3"
+        what, d = "linear_e4m3", self._device_index
         M, K = self._operand(what, "x", x, _E4M3).shape
-        N, Kw = self._operand(what, "w", w, _E4M3).shape
-        if Kw != K:
-            raise KernelError(f"{what}: rows of {K} values and weight rows of {Kw}")
-        self._operand(what, "x_scales", x_scales, _FLOAT, (M,), dense=True)
-        self._operand(what, "w_scales", w_scales, _FLOAT, (N,), dense=True)
-        self._product_places(what, x, N, out, _FLOATS)
+        if not (x_scales.get_device() == d == w.get_device() and w_scales.get_device() == d == out.get_device() and w.dtype is _F8
+                and x_scales.dtype is _F32T and w_scales.dtype is _F32T and out.dtype in _FLOATS and w.dim() == 2 and w.shape[1] == K
+                and x_scales.shape == (M,) and w_scales.shape == w.shape[:1] and out.shape == (M, w.shape[0])
+                and x_scales.is_contiguous() and w_scales.is_contiguous() and out.is_contiguous() and w.is_contiguous()):
+            N, width = self._operand(what, "w", w, _E4M3).shape
+            if width != K:
+                raise KernelError(f"{what}: rows of {K} values and weight rows of {width}")
+            self._operand(what, "x_scales", x_scales, _FLOAT, (M,), dense=True)
+            self._operand(what, "w_scales", w_scales, _FLOAT, (N,), dense=True)
+            self._operand(what, "out", out, _FLOATS, (M, N))
+        N = w.shape[0]
         if M and N:
-            fn = self._entry("gemm_e4m3", "llme_gemm_e4m3", c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int)
+            fn = self._typed.get("llme_gemm_e4m3") or self._entry("gemm_e4m3", "llme_gemm_e4m3", c_void_p, c_longlong, c_void_p, c_void_p, c_longlong,
+                                                                  c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int)
             self._launch("gemm_e4m3", what, fn, x.data_ptr(), self._row_stride(x), x_scales.data_ptr(), w.data_ptr(), self._row_stride(w),
                          w_scales.data_ptr(), out.data_ptr(), _code(out.dtype), self._row_stride(out), M, N, K)
         return out
@@ -697,20 +713,24 @@ class CudaOps:
         uint8 [N, ceil(K / 128) * 64], the codes c as weights.quantize.pack_int4 lays them; scales [N, ceil(K / group)] bfloat16 for a
         group of 32, 64 or 128; zeros uint8 of that shape with values 0..15 (None: 8 everywhere).  Sums are 32-bit.  K is a multiple
         of 8, the rows of x and w begin on 16 bytes (any such row stride)."""
-        what = "linear_int4"
+        what, d = "linear_int4", self._device_index
         M, K = self._operand(what, "x", x, _BF16S).shape
-        N, width = self._operand(what, "w", w, _BYTES).shape
-        if width != -(-K // 128) * 64:
-            raise KernelError(f"{what}: {K} codes a row take {-(-K // 128) * 64} bytes, w has {width}")
-        rows, groups = self._operand(what, "scales", scales, _BF16S, dense=True).shape
-        if rows != N:
-            raise KernelError(f"{what}: {N} weight rows and scales for {rows}")
+        if not (w.get_device() == d == scales.get_device() and out.get_device() == d and w.dtype is _BYTE and scales.dtype is _BF16T
+                and out.dtype is _BF16T and w.dim() == 2 == scales.dim() and w.shape[0] == scales.shape[0] and w.shape[1] == (K + 127) // 128 * 64
+                and out.shape == (M, w.shape[0]) and w.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
+            N, width = self._operand(what, "w", w, _BYTES).shape
+            if width != (K + 127) // 128 * 64:
+                raise KernelError(f"{what}: {K} codes a row take {(K + 127) // 128 * 64} bytes, w has {width}")
+            if self._operand(what, "scales", scales, _BF16S, dense=True).shape[0] != N:
+                raise KernelError(f"{what}: {N} weight rows and scales for {scales.shape[0]}")
+            self._operand(what, "out", out, _BF16S, (M, N))
+        N, groups = scales.shape
         if zeros is not None:
             self._operand(what, "zeros", zeros, _BYTES, (N, groups), dense=True)
-        group = self.int4_group(K, groups)
-        self._product_places(what, x, N, out, _BF16S)
+        group = 128 if groups == (K + 127) // 128 and K > 64 else self.int4_group(K, groups)
         if M and N:
-            fn = self._entry("gemm_int4", "llme_gemm_int4", c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_int, c_int)
+            fn = self._typed.get("llme_gemm_int4") or self._entry("gemm_int4", "llme_gemm_int4", c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
+                                                                  c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_int, c_int)
             self._launch("gemm_int4", what, fn, x.data_ptr(), self._row_stride(x), w.data_ptr(), self._row_stride(w), scales.data_ptr(), _ptr(zeros),
                          groups, group, out.data_ptr(), self._row_stride(out), M, N, K)
         return out
