@@ -25,8 +25,11 @@ namespace {
 #include "umma.cuh"
 #include "gemm_wide.cuh"
 #include "weight_stream.cuh"
+#include "gemm_int4_pair.cuh"
 
 constexpr int BLOCK_K = 128, BLOCK_BYTES = 64;
+
+int g_form = 0;                   // llme_gemm_int4_form()
 
 struct Args {
     const bf16* x; long long ldx;
@@ -231,18 +234,26 @@ int launch_skinny(const Args& a, cudaStream_t s) {
     return by.warps == 4 ? launch_skinny<MT, RUNS, ZEROS, 4, 24>(a, s) : launch_skinny<MT, RUNS, ZEROS, 2, 24>(a, s);
 }
 
-// More tokens than the weight-streaming kernel takes at once.
+// More tokens than the weight-streaming kernel takes at once: pairs of SMs, or single ones with K cut over a cluster, whichever a model of its
+// time says is faster.
 template <int RUNS, bool ZEROS>
 int launch_wide(const Args& a, cudaStream_t s) {
+    const long long w_bytes = (a.K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES;
+    alignas(64) CUtensorMap mw, mx;
+    if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
     wide::Args g{};
     g.out = a.out; g.ldo = a.ldo;
     g.M = a.M; g.N = a.N; g.K = a.K;
     g.scales = a.scales; g.zeros = a.zeros; g.lds = a.lds;
     g.vec_out = (uintptr_t)a.out % 8 == 0 && a.ldo % 4 == 0;
-    if (int rc = wide::shape<true, RUNS, ZEROS>(g, nullptr)) return rc;
-    const long long w_bytes = (a.K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES;
-    alignas(64) CUtensorMap mw, mx;
-    if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+    double single, paired;
+    if (int rc = wide::shape<true, RUNS, ZEROS>(g, &single)) return rc;
+    pair::PairArgs p{a.out, a.ldo, a.M, a.N, a.K, 0, 0, 0, a.scales, a.zeros, a.lds};
+    if (int rc = pair::shape<RUNS, ZEROS>(p, &paired)) return rc;
+    if (g_form == 2 || (g_form == 0 && paired < single)) {
+        if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, p.nt / 2, 64)) return rc;
+        return pair::launch<RUNS, ZEROS>(mw, mx, p, s);
+    }
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, g.nt, 64)) return rc;
     return wide::launch<true, RUNS, ZEROS>(mw, mx, g, s);
 }
@@ -279,6 +290,13 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     if (group == 32) return launch<1>(a, stream);
     if (group == 64) return launch<2>(a, stream);
     return launch<4>(a, stream);
+}
+
+// More than 16 tokens: 0 (the default): whichever kernel should be faster; 1: single SMs, K cut over clusters; 2: pairs of SMs.  For tests and
+// measurements.
+LLME_API int llme_gemm_int4_form(int how) {
+    if (how >= 0 && how <= 2) g_form = how;
+    return g_form;
 }
 
 // 0 if no bounded wait has given up since the last call (synchronises the device).

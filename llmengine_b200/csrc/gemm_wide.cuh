@@ -90,6 +90,15 @@ struct Group {
             bias[g] = *reinterpret_cast<const __nv_bfloat162*>(&b);
         }
     }
+    // a word's eight numbers, in order, of its group g
+    __device__ __forceinline__ void numbers(unsigned word, int g, unsigned* v) const {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const unsigned code = ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u;
+            const __nv_bfloat162 w = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&code), bias[g]), scale[g]);
+            v[p] = *reinterpret_cast<const unsigned*>(&w);
+        }
+    }
 };
 
 // INT4: bfloat16 tokens and 4-bit weights; else both e4m3.
@@ -208,13 +217,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             for (int j = 0; j < 4; ++j) {
                 unsigned v[16];
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        const unsigned code = ((words[q][j] >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-                        const __nv_bfloat162 w = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&code), now.bias[j / RUNS]), now.scale[j / RUNS]);
-                        v[q * 4 + p] = *reinterpret_cast<const unsigned*>(&w);
-                    }
+                for (int q = 0; q < 4; ++q) now.numbers(words[q][j], j / RUNS, v + q * 4);
                 tmem_store16(mine + (unsigned)(s * 64 + j * 16), v);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -340,8 +343,8 @@ int clusters_held(int segments, int per_sm) {
 
 // Tile width, segments, blocks an SM and stages of a product: what a model of its time says is least, in cycles.  The blocks that run at once
 // (as many as are held) share the memory's 2,900 bytes a cycle for the weights; an SM's blocks share its 42 bytes a cycle from L2 and its
-// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16).  Starting and ending a block cost about 5,500
-// cycles, the cluster's sums 1,000 and a little for every token.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
+// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16).  Starting and ending a block cost about 5,000
+// cycles and 14 for every token, the cluster's sums 1,000 and 4.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
 // 19.2 us, both in segments of four.)
 template <bool INT4, int RUNS, bool ZEROS>
 int shape(Args& g, double* cycles) {
@@ -363,7 +366,7 @@ int shape(Args& g, double* cycles) {
                 double step = share * (INT4 ? 4.0 : 2.0) * nt;
                 if (step < share * (w_bytes + nt * x_width) / 42.0) step = share * (w_bytes + nt * x_width) / 42.0;
                 if (step < at_once * w_bytes / 2900.0) step = at_once * w_bytes / 2900.0;
-                const double cost = rounds * (each * step + 5500.0 + (segments > 1 ? 1000.0 + 4.0 * nt : 0.0));
+                const double cost = rounds * (each * step + 5000.0 + 14.0 * nt + (segments > 1 ? 1000.0 + 4.0 * nt : 0.0));
                 if (best < 0.0 || cost < best) { best = cost; g.nt = nt; g.segments = segments; g.segment_steps = each; g.per_sm = per_sm; }
             }
     }

@@ -693,10 +693,12 @@ class CudaOps:
                          w_scales.data_ptr(), out.data_ptr(), _code(out.dtype), self._row_stride(out), M, N, K)
         return out
 
-    def linear_e4m3_form(self, how: str) -> None:
-        """Which kernel multiplies more than 16 rows by 8-bit weights: "auto" (the one that should be faster), "wide" (narrow tiles, K cut
-        over clusters) or "pair" (256 x 256 tiles on pairs of SMs).  For tests and measurements."""
-        self._lib("gemm_e4m3").llme_gemm_e4m3_form(c_int({"auto": 0, "wide": 1, "pair": 2}[how]))
+    def low_bit_form(self, how: str) -> None:
+        """Which kernels multiply more than 16 rows by weights of 8 and 4 bits: "auto" (those that should be faster), "wide" (the weights on
+        the lanes of one SM's tensor memory, K cut over clusters) or "pair" (tiles on pairs of SMs).  For tests and measurements."""
+        code = c_int({"auto": 0, "wide": 1, "pair": 2}[how])
+        self._lib("gemm_e4m3").llme_gemm_e4m3_form(code)
+        self._lib("gemm_int4").llme_gemm_int4_form(code)
 
     @staticmethod
     def int4_group(k: int, groups: int) -> int:

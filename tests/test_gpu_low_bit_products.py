@@ -53,11 +53,11 @@ def _exact_e4m3(x, xs, w, ws):
 
 
 @pytest.fixture(params=["wide", "pair", "auto"])
-def e4m3(ops, request):
-    """The product of 8-bit rows also by the kernel that its own choice would not take."""
-    ops.linear_e4m3_form(request.param)
+def forms(ops, request):
+    """The products of more than 16 rows also by the kernel that their own choice would not take."""
+    ops.low_bit_form(request.param)
     yield ops
-    ops.linear_e4m3_form("auto")
+    ops.low_bit_form("auto")
 
 
 M_SIZES = [1, 2, 8, 9, 16, 17, 24, 33, 64, 77, 128, 129, 200, 256, 257, 513]
@@ -65,13 +65,13 @@ M_SIZES = [1, 2, 8, 9, 16, 17, 24, 33, 64, 77, 128, 129, 200, 256, 257, 513]
 
 @pytest.mark.parametrize("m", M_SIZES)
 @pytest.mark.parametrize("n,k", [(1, 16), (8, 128), (100, 144), (129, 4096), (1000, 272), (2048, 1040), (264, 12288)])
-def test_e4m3_places(e4m3, m, n, k):
+def test_e4m3_places(forms, m, n, k):
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=m + n + k)
     want = _exact_e4m3(x, xs, w, ws)
     for dtype in (torch.float32, torch.bfloat16):
         for extra in (0, 5):
             whole, out = _out(m, n, dtype, extra)
-            assert e4m3.linear_e4m3(x, xs, w, ws, out) is out
+            assert forms.linear_e4m3(x, xs, w, ws, out) is out
             assert torch.equal(out.double(), want.to(dtype).double())
             _rest_untouched(whole, n)
 
@@ -79,19 +79,19 @@ def test_e4m3_places(e4m3, m, n, k):
 @pytest.mark.parametrize("m", [1, 8, 16, 40, 77, 128, 300, 1024])
 @pytest.mark.parametrize("n,k", [(512, 4096), (264, 12288), (4096, 528)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_e4m3_rounding(e4m3, m, n, k, dtype):
+def test_e4m3_rounding(forms, m, n, k, dtype):
     from llmengine_b200.weights.quantize import quantize_e4m3
     g = _gen(m + n)
     x, xs = quantize_e4m3((torch.randn(m, k, generator=g) * 3).to(DEV))
     w, ws = quantize_e4m3((torch.randn(n, k, generator=g) * 0.02).to(DEV))
     _, out = _out(m, n, dtype)
-    e4m3.linear_e4m3(x, xs, w, ws, out)
+    forms.linear_e4m3(x, xs, w, ws, out)
     want, size = _exact_e4m3(x, xs, w, ws), _exact_e4m3(x.float().abs(), xs, w.float().abs(), ws)
     assert torch.all((out.double() - want).abs() <= _bound(dtype, want, size, k))
 
 
 @pytest.mark.parametrize("m", [3, 16, 40, 130, 300])
-def test_e4m3_strides(e4m3, m):
+def test_e4m3_strides(forms, m):
     """Operands that are columns and rows of larger matrices."""
     n, k = 200, 400
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=m)
@@ -102,13 +102,13 @@ def test_e4m3_strides(e4m3, m):
     big_w.view(torch.uint8)[:2] = 0x7F
     big_w.view(torch.uint8)[2 + n:] = 0x7F
     whole, out = _out(m, n, torch.bfloat16, 8)
-    e4m3.linear_e4m3(big_x[:, 32:32 + k], xs, big_w[2:2 + n, :k], ws, out)
+    forms.linear_e4m3(big_x[:, 32:32 + k], xs, big_w[2:2 + n, :k], ws, out)
     assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws).to(torch.bfloat16).double())
     _rest_untouched(whole, n)
 
 
 @pytest.mark.parametrize("m", [4, 16, 40, 200, 300])
-def test_e4m3_rows_that_are_no_numbers(e4m3, m):
+def test_e4m3_rows_that_are_no_numbers(forms, m):
     n, k = 300, 512
     x, xs, w, ws = _whole_e4m3(m, n, k, seed=1)
     clean = _exact_e4m3(x, xs, w, ws)
@@ -117,7 +117,7 @@ def test_e4m3_rows_that_are_no_numbers(e4m3, m):
     x.view(torch.uint8)[2, 5] = 0x7F
     w.view(torch.uint8)[250, 3] = 0xFF
     _, out = _out(m, n, torch.float32)
-    e4m3.linear_e4m3(x, xs, w, ws, out)
+    forms.linear_e4m3(x, xs, w, ws, out)
     bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
     bad[1:3] = True
     bad[:, 250] = True
@@ -145,13 +145,13 @@ def _weights64(codes, scales, zero, group):
 @pytest.mark.parametrize("m", M_SIZES)
 @pytest.mark.parametrize("n,k", [(1, 8), (8, 128), (100, 136), (129, 4096), (1000, 264), (2048, 1000), (264, 12288)])
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
-def test_int4_places(ops, m, n, k, group, zeros):
+def test_int4_places(forms, m, n, k, group, zeros):
     from llmengine_b200.weights.quantize import pack_int4
     x, codes, scales, zero = _whole_int4(m, n, k, group, zeros, seed=m + n + k)
     want = (x.double() @ _weights64(codes, scales, zero, group).t()).to(torch.bfloat16)
     for extra in (0, 5):
         whole, out = _out(m, n, torch.bfloat16, extra)
-        assert ops.linear_int4(x, pack_int4(codes), scales, out, zeros=zero) is out
+        assert forms.linear_int4(x, pack_int4(codes), scales, out, zeros=zero) is out
         assert torch.equal(out, want)
         _rest_untouched(whole, n)
 
@@ -159,20 +159,20 @@ def test_int4_places(ops, m, n, k, group, zeros):
 @pytest.mark.parametrize("m", [1, 8, 16, 40, 77, 128, 300, 1024])
 @pytest.mark.parametrize("n,k", [(512, 4096), (264, 12288), (4096, 520)])
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
-def test_int4_rounding(ops, m, n, k, group, zeros):
+def test_int4_rounding(forms, m, n, k, group, zeros):
     from llmengine_b200.weights.quantize import dequantize_int4, quantize_int4
     g = _gen(m + n)
     x = (torch.randn(m, k, generator=g) * 3).to(torch.bfloat16).to(DEV)
     packed, scales, zero = quantize_int4((torch.randn(n, k, generator=g) * 0.02).to(DEV), group, zeros)
     _, out = _out(m, n, torch.bfloat16)
-    ops.linear_int4(x, packed, scales, out, zeros=zero)
+    forms.linear_int4(x, packed, scales, out, zeros=zero)
     w = dequantize_int4(packed, scales, zero, k, group).double()
     want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
     assert torch.all((out.double() - want).abs() <= _bound(torch.bfloat16, want, size, k, 2.0 ** -8 if m > 16 else 0.0))
 
 
 @pytest.mark.parametrize("m", [3, 16, 40, 130, 300])
-def test_int4_strides(ops, m):
+def test_int4_strides(forms, m):
     from llmengine_b200.weights.quantize import pack_int4
     n, k, group = 200, 400, 64
     x, codes, scales, zero = _whole_int4(m, n, k, group, True, seed=m)
@@ -182,13 +182,13 @@ def test_int4_strides(ops, m):
     big_w = torch.full((n + 3, packed.shape[1] + 16), 0xFF, dtype=torch.uint8, device=DEV)
     big_w[2:2 + n, :packed.shape[1]] = packed
     whole, out = _out(m, n, torch.bfloat16, 8)
-    ops.linear_int4(big_x[:, 16:16 + k], big_w[2:2 + n, :packed.shape[1]], scales, out, zeros=zero)
+    forms.linear_int4(big_x[:, 16:16 + k], big_w[2:2 + n, :packed.shape[1]], scales, out, zeros=zero)
     assert torch.equal(out, (x.double() @ _weights64(codes, scales, zero, group).t()).to(torch.bfloat16))
     _rest_untouched(whole, n)
 
 
 @pytest.mark.parametrize("m", [4, 16, 40, 200, 300])
-def test_int4_rows_that_are_no_numbers(ops, m):
+def test_int4_rows_that_are_no_numbers(forms, m):
     from llmengine_b200.weights.quantize import pack_int4
     n, k = 300, 520
     x, codes, scales, _ = _whole_int4(m, n, k, 128, False, seed=1)
@@ -198,7 +198,7 @@ def test_int4_rows_that_are_no_numbers(ops, m):
     codes[:, 519], codes[7, 519] = 9, 8                             # infinity times 1, and once times 0
     _, out = _out(m, n, torch.bfloat16)
     before = x.clone()
-    ops.linear_int4(x, pack_int4(codes), scales, out)
+    forms.linear_int4(x, pack_int4(codes), scales, out)
     before[1:3] = 0
     clean = (before.double() @ _weights64(codes, scales.nan_to_num(1.0), None, 128).t()).to(torch.bfloat16)
     assert torch.isnan(out[1]).all() and torch.isnan(out[:, 250]).all() and torch.isnan(out[2, 7])
