@@ -344,7 +344,7 @@ int clusters_held(int segments, int per_sm) {
 // Tile width, segments, blocks an SM and stages of a product: what a model of its time says is least, in cycles.  The blocks that run at once
 // (as many as are held) share the memory's 2,900 bytes a cycle for the weights; an SM's blocks share its 42 bytes a cycle from L2 and its
 // tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16).  Starting and ending a block cost about 5,000
-// cycles and 14 for every token, the cluster's sums 1,000 and 4.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
+// cycles and 14 for every token, the cluster's sums 1,000 and 16.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
 // 19.2 us, both in segments of four.)
 template <bool INT4, int RUNS, bool ZEROS>
 int shape(Args& g, double* cycles) {
@@ -366,7 +366,7 @@ int shape(Args& g, double* cycles) {
                 double step = share * (INT4 ? 4.0 : 2.0) * nt;
                 if (step < share * (w_bytes + nt * x_width) / 42.0) step = share * (w_bytes + nt * x_width) / 42.0;
                 if (step < at_once * w_bytes / 2900.0) step = at_once * w_bytes / 2900.0;
-                const double cost = rounds * (each * step + 5000.0 + 14.0 * nt + (segments > 1 ? 1000.0 + 4.0 * nt : 0.0));
+                const double cost = rounds * (each * step + 5000.0 + 14.0 * nt + (segments > 1 ? 1000.0 + 16.0 * nt : 0.0));
                 if (best < 0.0 || cost < best) { best = cost; g.nt = nt; g.segments = segments; g.segment_steps = each; g.per_sm = per_sm; }
             }
     }
