@@ -85,10 +85,12 @@ template <int N> __device__ __forceinline__ void store_e4m3(unsigned char* p, co
     }
 }
 
+inline int least(int a, int b) { return a < b ? a : b; }
+
 // ---- where a row comes from.  fetch() brings what N values at column j are made of, values() makes them.
 template <typename T> struct FromRows {
     static constexpr bool NORM = false, EXACT = true;
-    static constexpr int MOST = 4;                 // pieces of eight values a thread holds where rows are many
+    static int many(int pieces) { return least(sizeof(T) == 2 ? 4 : 2, pieces / 128); }      // pieces a thread holds where rows are many
     const T* x; long long ldx;
     template <int N> using Raw = Piece<T, N>;
     template <int N> __device__ __forceinline__ void fetch(int row, int j, Raw<N>& r) const { r.load(x + row * ldx + j); }
@@ -97,9 +99,18 @@ template <typename T> struct FromRows {
         for (int i = 0; i < N; ++i) v[i] = r.at(i);
     }
 };
+// 1 / (1 + exp(-g)) for a g that has been through bfloat16, from the hardware's exponential and reciprocal: 2^-22 and 2^-23 of the value (and the
+// rounding of the exponent), far below the 2^-4 of what it goes into.  Arithmetic bounds the gate's kernel: with the corrected reciprocal and
+// the exponential for subnormal results 2,048 x 17,408 took 39.0 us.
+__device__ __forceinline__ float sigmoid_fast(float g) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
 template <typename T> struct FromGate {
     static constexpr bool NORM = false, EXACT = false;
-    static constexpr int MOST = 6;
+    static int many(int pieces) { return sizeof(T) == 4 ? 1 : (pieces <= 3 * 512 ? least(3, pieces / 128) : 6); }
     const T* x; long long ldx; int inter;
     template <int N> struct Raw { Piece<T, N> gate, up; };
     template <int N> __device__ __forceinline__ void fetch(int row, int j, Raw<N>& r) const {
@@ -110,14 +121,14 @@ template <typename T> struct FromGate {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float g = r.gate.at(i);
-            v[i] = sizeof(T) == 2 ? silu_mul_bf16(g, r.up.at(i)) : g / (1.0f + expf(-g)) * r.up.at(i);
+            v[i] = (sizeof(T) == 2 ? g * sigmoid_fast(g) : g / (1.0f + expf(-g))) * r.up.at(i);
         }
     }
 };
 // D: type of the contribution, or void where none is pending
 template <typename D, typename G> struct FromNorm {
     static constexpr bool NORM = true, EXACT = false;
-    static constexpr int MOST = 1;                 // (a row's squares are added in an order that must not depend on how many rows there are)
+    static int many(int) { return 1; }             // (a row's squares are added in an order that must not depend on how many rows there are)
     const float* x; const D* delta; const G* gain; float* total; int size; float eps;
     template <int N> using Gain = Piece<G, N>;
     template <int N> struct Raw {
@@ -139,8 +150,12 @@ template <typename D, typename G> struct FromNorm {
     }
 };
 
-// The largest of several |v| as bits: for numbers without a sign they are in the order of the values, infinity above all, NaN above that.
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The larger of `top` and |v|, NaN if either is one; for numbers without a sign the order of the values is that of their bits, infinity above
+// all, NaN above that.
+__device__ __forceinline__ float larger(float top, float v) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v)));
+    return top;
+}
 
 // v / a from 1 / a and one correction: the quotient's error is known exactly, v - q a.  (Values of a few bits over a scale of theirs meet the
 // middle between two e4m3 numbers often, and v times 1 / a would fall to either side of it.)
@@ -150,22 +165,24 @@ __device__ __forceinline__ float quotient(float v, float a, float f) {
 }
 
 // A row's scale and the factor that takes its values to e4m3: `top` the largest |h| before it is multiplied by r.
-__device__ __forceinline__ float row_scale(unsigned top, float r) {
-    const float m = __uint_as_float(top) * r;
+__device__ __forceinline__ float row_scale(float top, float r) {
+    const float m = top * r;
     return (m >= LEAST ? m : (m < LEAST ? LEAST : m)) / LARGEST;       // (NaN stays)
 }
 
 // Sum and largest over the threads of a row: the lanes of a warp, or a block's.
 template <bool BLOCK>
-__device__ __forceinline__ void meet(float& ss, unsigned& top, float* sums, unsigned* tops) {
+__device__ __forceinline__ void meet(float& ss, float& top, float* sums, unsigned* tops) {
     ss = warp_sum(ss);
-    top = __reduce_max_sync(0xffffffffu, top);
+    unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    top = __uint_as_float(bits);
     if (!BLOCK) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if (lane == 0) { sums[warp] = ss; tops[warp] = top; }
+    if (lane == 0) { sums[warp] = ss; tops[warp] = bits; }
     __syncthreads();
     ss = warp_sum(lane < warps ? sums[lane] : 0.0f);
-    top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+    bits = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+    top = __uint_as_float(bits);
 }
 
 // BLOCK: a block a row; else a warp a row.  V: pieces of N values a thread holds.
@@ -182,8 +199,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
 #pragma unroll
     for (int k = 0; k < V; ++k)
         if ((t + k * step) * N < size) src.template fetch<N>(row, (t + k * step) * N, raw[k]);
-    float v[V][N], ss = 0.0f;
-    unsigned top = 0;
+    float v[V][N], ss = 0.0f, top = 0.0f;
     if constexpr (Src::NORM) {
         typename Src::template Gain<N> gain[V];
 #pragma unroll
@@ -197,7 +213,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 ss = fmaf(v[k][i], v[k][i], ss);
-                top = max(top, magnitude(v[k][i] * gain[k].at(i)));
+                top = larger(top, v[k][i] * gain[k].at(i));
             }
         }
         meet<BLOCK>(ss, top, sums, tops);
@@ -218,7 +234,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
             if (j >= size) continue;
             src.template values<N>(row, j, raw[k], v[k]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) top = max(top, magnitude(v[k][i]));
+            for (int i = 0; i < N; ++i) top = larger(top, v[k][i]);
         }
         meet<BLOCK>(ss, top, sums, tops);
         const float a = row_scale(top, 1.0f), f = 1.0f / a;
@@ -244,8 +260,7 @@ __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsig
     pdl_wait();
     const int row = (int)blockIdx.x;
     typename Src::template Raw<1> raw;
-    float ss = 0.0f, v[1];
-    unsigned top = 0;
+    float ss = 0.0f, top = 0.0f, v[1];
     for (int j = (int)threadIdx.x; j < size; j += (int)blockDim.x) {
         src.template fetch<1>(row, j, raw);
         src.template values<1>(row, j, raw, v);
@@ -253,7 +268,7 @@ __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsig
             ss = fmaf(v[0], v[0], ss);
             v[0] *= to_f32(src.gain[j]);
         }
-        top = max(top, magnitude(v[0]));
+        top = larger(top, v[0]);
     }
     meet<true>(ss, top, sums, tops);
     float r = 1.0f;
@@ -289,18 +304,20 @@ int sm_count() {
 
 // `vec`: the widest pieces that every operand takes.
 // Few rows: as many threads a row as it has pieces of eight values, for the shortest way through.  Rows for several rounds of the SMs: several
-// pieces a thread, so that more rows are on an SM at once and one's loads run while another's threads meet (4,096 rows of 4,096 bfloat16
-// values, 1 / 2 / 4 / 6 pieces a thread: 13.9 / 11.7 / 10.6 / 10.9 us; the gate, 2,048 x 17,408: 62.5 with 4, 39.2 with 6, which leaves room for two
-// blocks an SM; the norm, 2,048 x 4,096 with a 32-bit contribution, gains nothing: 18.0 / 17.9 / 19.3 / 25.3), but no fewer than 128 threads (2,048
-// rows of 1,024: 3.4 us with 1, 3.7 with 2).
+// pieces a thread, so that more rows are on an SM at once and one's loads run while another's threads meet, as far as the registers of two and
+// more blocks an SM go (1 / 2 / 3 / 4 / 6 pieces a thread: 4,096 rows of 4,096 bfloat16 values 13.4 / 11.1 / 10.7 / 10.2 / 10.5 us; the gate of
+// 2,048 x 5,504 14.7 / 11.2 / 11.1 / 12.9 / 12.1, of 12,288 - / 22.8 / 22.8 / 26.9 / 22.4, of 17,408 - / - / - / 51.5 / 31.4, of 8,192 in 32 bits
+// 24.9 / 27.1 / 30.3 / 33.6 / 41.6; the norm, 1,999 x 5,120, 18.7 / 18.7 / 19.2 / 20.4 / 23.0), but no fewer than 128 threads.  (A walk of as
+// many blocks as fit, the next row's loads under way in shared memory, was slower throughout: 15.2 to 11.6 us for the first, 42.3 for 17,408.)
 template <class Src>
 int launch(const Src& src, unsigned char* q, long long ldq, float* scales, int rows, int size, int vec, cudaStream_t s) {
     const int pieces = size / vec;
-    int v = rows >= 2 * sm_count() ? (pieces / 128 < Src::MOST ? pieces / 128 : Src::MOST) : 1;
+    int v = rows >= 2 * sm_count() ? Src::many(pieces) : 1;
     while (v > 1 ? pieces > v * 640 : pieces > 1024) ++v;
     if (vec == 8 && pieces <= 32) llme_launch(quantise_kernel<Src, 8, 1, false>, dim3((rows + 3) / 4), dim3(128), 0, s, src, q, ldq, scales, rows, size);
     else if (vec == 8 && v <= 1) launch_block<Src, 8, 1>(src, q, ldq, scales, rows, size, s);
     else if (vec == 8 && v <= 2) launch_block<Src, 8, 2>(src, q, ldq, scales, rows, size, s);
+    else if (vec == 8 && v <= 3) launch_block<Src, 8, 3>(src, q, ldq, scales, rows, size, s);
     else if (vec == 8 && v <= 4) launch_block<Src, 8, 4>(src, q, ldq, scales, rows, size, s);
     else if (vec == 8 && v <= 6) launch_block<Src, 8, 6>(src, q, ldq, scales, rows, size, s);
     else if (vec >= 2 && size / 2 <= 8 * 640) launch_block<Src, 2, 8>(src, q, ldq, scales, rows, size, s);
