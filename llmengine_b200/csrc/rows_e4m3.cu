@@ -250,40 +250,48 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
     }
 }
 
-// Any width and alignment: the row is read a second time.  (A norm's second pass reads the sums that the first one wrote: the same
-// thread's.)
-template <class Src>
+// Any width and alignment, N values at a time (2 or 1): the row is read a second time.  (A norm's second pass reads the sums that the first one
+// wrote: the same thread's.)
+template <class Src, int N>
 __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsigned char* __restrict__ q, long long ldq, float* __restrict__ scales, int rows, int size) {
     __shared__ float sums[32];
     __shared__ unsigned tops[32];
     pdl_launch_dependents();
     pdl_wait();
     const int row = (int)blockIdx.x;
-    typename Src::template Raw<1> raw;
-    float ss = 0.0f, top = 0.0f, v[1];
-    for (int j = (int)threadIdx.x; j < size; j += (int)blockDim.x) {
-        src.template fetch<1>(row, j, raw);
-        src.template values<1>(row, j, raw, v);
-        if constexpr (Src::NORM) {
-            ss = fmaf(v[0], v[0], ss);
-            v[0] *= to_f32(src.gain[j]);
+    float ss = 0.0f, top = 0.0f, v[N];
+    for (int j = N * (int)threadIdx.x; j < size; j += N * (int)blockDim.x) {
+        typename Src::template Raw<N> raw;
+        src.template fetch<N>(row, j, raw);
+        src.template values<N>(row, j, raw, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (Src::NORM) {
+                ss = fmaf(v[i], v[i], ss);
+                v[i] *= to_f32(src.gain[j + i]);
+            }
+            top = larger(top, v[i]);
         }
-        top = larger(top, v[0]);
     }
     meet<true>(ss, top, sums, tops);
     float r = 1.0f;
     if constexpr (Src::NORM) r = 1.0f / sqrtf(ss / (float)size + src.eps);
     const float a = row_scale(top, r), f = r / a;
     if (threadIdx.x == 0) scales[row] = a;
-    for (int j = (int)threadIdx.x; j < size; j += (int)blockDim.x) {
+    for (int j = N * (int)threadIdx.x; j < size; j += N * (int)blockDim.x) {
         if constexpr (Src::NORM) {
-            v[0] = ((src.delta ? src.total : src.x)[(long long)row * size + j] * f) * to_f32(src.gain[j]);
+            Piece<float, N> t;
+            t.load((src.delta ? src.total : src.x) + (long long)row * size + j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (t.at(i) * f) * to_f32(src.gain[j + i]);
         } else {
-            src.template fetch<1>(row, j, raw);
-            src.template values<1>(row, j, raw, v);
-            v[0] = Src::EXACT ? quotient(v[0], a, f) : v[0] * f;
+            typename Src::template Raw<N> raw;
+            src.template fetch<N>(row, j, raw);
+            src.template values<N>(row, j, raw, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = Src::EXACT ? quotient(v[i], a, f) : v[i] * f;
         }
-        store_e4m3<1>(q + row * ldq + j, v);
+        store_e4m3<N>(q + row * ldq + j, v);
     }
 }
 
@@ -321,7 +329,8 @@ int launch(const Src& src, unsigned char* q, long long ldq, float* scales, int r
     else if (vec == 8 && v <= 4) launch_block<Src, 8, 4>(src, q, ldq, scales, rows, size, s);
     else if (vec == 8 && v <= 6) launch_block<Src, 8, 6>(src, q, ldq, scales, rows, size, s);
     else if (vec >= 2 && size / 2 <= 8 * 640) launch_block<Src, 2, 8>(src, q, ldq, scales, rows, size, s);
-    else llme_launch(quantise_long_kernel<Src>, dim3(rows), dim3(size >= 2048 ? 512 : 128), 0, s, src, q, ldq, scales, rows, size);
+    else if (vec >= 2) llme_launch(quantise_long_kernel<Src, 2>, dim3(rows), dim3(512), 0, s, src, q, ldq, scales, rows, size);
+    else llme_launch(quantise_long_kernel<Src, 1>, dim3(rows), dim3(size >= 2048 ? 512 : 128), 0, s, src, q, ldq, scales, rows, size);
     LLME_LAUNCH_STATUS();
 }
 
