@@ -67,3 +67,12 @@ def test_generation_with_captured_steps(tmp_path, form):
         outs.append([o.token_ids for o in llm.generate(prompts, SamplingParams(greedy=True), max_tokens=24)])
         del llm
     assert outs[0] == outs[1] and all(len(t) > 0 for t in outs[0])
+
+
+@pytest.mark.parametrize("flags", [["--weights", "e4m3"], ["--weights", "int4", "--weight-group", "64", "--weight-zero-points"]])
+def test_the_command(tmp_path, capsys, flags):
+    from llmengine_b200.generate import main
+    folder = make_model_dir(str(tmp_path), TINY_D, seed=4)
+    assert main([folder, "5,17,3", "6", "--ignore-eos", "--greedy", "--max-cached-tokens", "512", *flags]) == 0
+    out = capsys.readouterr().out.splitlines()
+    assert len(out[0].split()) == 6 and "[Generated 6 tokens total]" in out

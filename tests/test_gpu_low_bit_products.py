@@ -294,3 +294,61 @@ def test_operands_side_by_side(ops):
     out = both[:, 64:].view(torch.float32)
     ops.linear_e4m3(both[:, :64].view(F8), xs, w, ws, out)
     assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws)) and torch.equal(both[:, :64], x.view(torch.uint8))
+
+
+@pytest.mark.parametrize("m", [8, 40, 700])
+def test_two_streams_at_once(ops, m):
+    """Calls on two streams, whose blocks may share SMs and their tensor memory, each give what one alone gives."""
+    from llmengine_b200.weights.quantize import pack_int4
+    n, k = 520, 2048
+    a, b = _whole_e4m3(m, n, k, seed=7), _whole_int4(m, n, k, 64, True, seed=8)
+    packed = pack_int4(b[1])
+    want8, want4 = _exact_e4m3(*a).float(), (b[0].double() @ _weights64(b[1], b[2], b[3], 64).t()).to(torch.bfloat16)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[(torch.empty(m, n, device=DEV), torch.empty(m, n, dtype=torch.bfloat16, device=DEV)) for _ in range(20)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, mine in zip(streams, outs):
+            with torch.cuda.stream(s):
+                ops.linear_e4m3(*a, mine[i][0])
+                ops.linear_int4(b[0], packed, b[2], mine[i][1], zeros=b[3])
+    torch.cuda.synchronize()
+    for mine in outs:
+        for out8, out4 in mine:
+            assert torch.equal(out8, want8) and torch.equal(out4, want4)
+
+
+@pytest.mark.parametrize("m", [9, 40, 300])
+def test_outputs_behind_32_bits(ops, m):
+    """Output rows so far apart that the last ones begin behind 2^31 values."""
+    from llmengine_b200.weights.quantize import pack_int4
+    n, k, stride = 136, 256, (1 << 31) // (m - 2)
+    stride += -stride % 8
+    a, b = _whole_e4m3(m, n, k, seed=9), _whole_int4(m, n, k, 128, False, seed=10)
+    whole = torch.empty(m * stride, dtype=torch.bfloat16, device=DEV)
+    for extra in (0, 3):                                            # rows that begin on 16 bytes, and that do not
+        out = whole[extra:].as_strided((m, n), (stride, 1))
+        out.fill_(5.0)
+        ops.linear_e4m3(*a, out)
+        assert torch.equal(out, _exact_e4m3(*a).to(torch.bfloat16))
+        out.fill_(5.0)
+        ops.linear_int4(b[0], pack_int4(b[1]), b[2], out)
+        assert torch.equal(out, (b[0].double() @ _weights64(b[1], b[2], None, 128).t()).to(torch.bfloat16))
+
+
+def test_operands_behind_32_bits(ops):
+    """Rows and weights whose last ones begin behind 2^31 bytes and values."""
+    n, k = 40, 64
+    for m in (16, 40, 300):
+        x, xs, w, ws = _whole_e4m3(m, n, k, seed=11)
+        big = torch.zeros(2200000000, dtype=torch.uint8, device=DEV)
+        sx, sw = 2199990000 // m // 16 * 16, 2199990000 // n // 16 * 16
+        out = torch.empty(m, n, device=DEV)
+        far = big.as_strided((m, k), (sx, 1))
+        far.copy_(x.view(torch.uint8))
+        ops.linear_e4m3(far.view(F8), xs, w, ws, out)
+        assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws))
+        far = big.as_strided((n, k), (sw, 1))
+        far.copy_(w.view(torch.uint8))
+        ops.linear_e4m3(x, xs, far.view(F8), ws, out)
+        assert torch.equal(out.double(), _exact_e4m3(x, xs, w, ws))

@@ -220,3 +220,17 @@ def test_refusals(ops):
             call()
             print("not refused:", i)
     assert ops.launches == n
+
+
+def test_rows_behind_32_bits(ops):
+    """More than 2^31 values: the last rows are read and written where they are."""
+    rows, size = 540000, 4096
+    x = torch.zeros(rows, size, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = _rand(3, size, dtype=torch.bfloat16, seed=13)
+    q, scales = torch.empty(rows, size, dtype=F8, device=DEV), torch.empty(rows, device=DEV)
+    ops.rows_e4m3(x, q, scales)
+    _check(x[-3:].double(), q[-3:], scales[-3:], D_ROWS)
+    assert torch.all(q[:-3].view(torch.uint8).amax(1) == 0)
+    ops.swiglu_e4m3(x.view(rows // 2, 2 * size), q[:rows // 2], scales[:rows // 2])
+    g, u = x[-2:].double()
+    _check((g * torch.sigmoid(g) * u)[None], q[rows // 2 - 1][None], scales[rows // 2 - 1][None], D_GATE)
