@@ -5,7 +5,8 @@
 // block loads its own 128 tokens' rows and half of the tile's weight rows, 128 values of K (one swizzle row) at a time, six stages deep; the
 // instructions, issued by the pair's first block alone, read both blocks' shared memory and add into both blocks' tensor memory, where the
 // accumulator is double-buffered.  Eight warps of each block read it back, multiply by the two scales and store through shared memory
-// (TMA; straight from registers where the output's rows do not begin on 16 bytes).  The plumbing is that of the bfloat16 product on pairs
+// (TMA; value by value where the output's rows do not begin on 16 bytes): 2048 x 24576 x 128, which is little else, 29 us in bfloat16 and
+// 37 in 32 bits (5.4 TB/s of output); rows of an odd length, 2048 x 10423 x 2576 in bfloat16, 58 us, straight from registers 256.  The plumbing is that of the bfloat16 product on pairs
 // (gemm_tcgen05.cu); a step moves the same bytes and does twice the work.
 #pragma once
 
@@ -42,7 +43,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int steps = (a.K + STEP - 1) / STEP, m_tiles = (a.M + TILE_M - 1) / TILE_M, n_tiles = (a.N + BN - 1) / BN;
-    const long long tiles = (long long)m_tiles * n_tiles;
+    const int tiles = m_tiles * n_tiles;             // (65,536 outputs each: fewer than 2^31 in any memory)
     const unsigned rank = cluster_rank();                              // 0: the block that issues the pair's instructions
     const int walker = (int)(blockIdx.x >> 1), walkers = (int)(gridDim.x >> 1);
 
@@ -73,8 +74,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         // ------------------------------------------------------------------ loads
         unsigned it = 0;
         bool ok = true;
-        for (long long t = walker; t < tiles && ok; t += walkers) {
-            const int m0 = (int)(t % m_tiles) * TILE_M + (int)rank * BM, n0 = (int)(t / m_tiles) * BN + (int)rank * (BN / 2);
+        for (int t = walker; t < tiles && ok; t += walkers) {
+            const int m0 = t % m_tiles * TILE_M + (int)rank * BM, n0 = t / m_tiles * BN + (int)rank * (BN / 2);
             for (int c = 0; c < steps; ++c, ++it) {
                 const unsigned s = it % STAGES;
                 ok = mbar_wait(&bar->empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, 11) && !*abort_flag;
@@ -106,7 +107,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             unsigned it = 0;
             bool ok = true;
             int i = 0;
-            for (long long t = walker; t < tiles && ok; t += walkers, ++i) {
+            for (int t = walker; t < tiles && ok; t += walkers, ++i) {
                 const int b = i & 1;
                 ok = mbar_wait(&bar->acc_empty[b], ((i >> 1) & 1) ^ 1, abort_flag, 14);      // the epilogue has drained this buffer
                 if (!ok) break;
@@ -131,69 +132,72 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     } else {
         // ------------------------------------------------------------------ the way out (warps 2..9: two for every 32 lanes, half of the columns each)
         const int quarter = warp & 3;             // the lanes of tensor memory this warp may read
-        constexpr int COLS = 128 / (int)sizeof(O);                     // output columns per 128-byte staging row
-        const int col0 = ((warp - 2) >> 2) * (BN / 2);
-        unsigned char* buf = staging + (warp - 2) * 4096;
+        constexpr int PIECES = (int)sizeof(O) / 2, COLS = 32 / PIECES;             // 64-byte pieces of 32 columns; columns of a piece
+        const int col0 = ((warp - 2) >> 2) * (BN / 2), swizzle = (lane >> 1) & 3;
+        unsigned char* own = staging + (warp - 2) * 4096;                              // two pieces of 32 rows x 64 bytes
         const unsigned acc_empty_first = map_to_cta(smem_u32(&bar->acc_empty[0]), 0);
         int i = 0;
-        for (long long t = walker; t < tiles; t += walkers, ++i) {
-            const int m0 = (int)(t % m_tiles) * TILE_M + (int)rank * BM, n0 = (int)(t / m_tiles) * BN, b = i & 1, row = m0 + quarter * 32 + lane;
+        for (int t = walker; t < tiles; t += walkers, ++i) {
+            const int m0 = t % m_tiles * TILE_M + (int)rank * BM + quarter * 32, n0 = t / m_tiles * BN + col0, b = i & 1, row = m0 + lane;
+            // (the scales are on their way while the tile is worked on: column `lane` of every 32, handed round below)
+            const float xs = row < a.M ? a.xs[row] : 0.0f;
+            float ws[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ws[j] = n0 + j * 32 + lane < a.N ? a.ws[n0 + j * 32 + lane] : 0.0f;
             if (!mbar_wait(&bar->acc_full[b], (i >> 1) & 1, abort_flag, 13)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float xs = row < a.M ? a.xs[row] : 0.0f;
-            const unsigned tmem_row = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(b * BN);
-#pragma unroll 1
-            for (int c = col0; c < col0 + BN / 2; c += COLS) {
-                if (TMA_STORE) {
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the store before has read the buffer
+            const unsigned mine = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(b * BN + col0);
+            unsigned v[2][32];
+            tmem_ld_32x32(mine, v[0]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unsigned (&f)[32] = v[j & 1];
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (j < 3) tmem_ld_32x32(mine + (unsigned)(j * 32 + 32), v[(j + 1) & 1]);
+                else {                                                                        // its half of the tile has left tensor memory
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
+                    if (lane == 0) wide::mbar_arrive_remote(acc_empty_first + (unsigned)(b * 8));
                 }
 #pragma unroll
-                for (int half = 0; half < COLS / 32; ++half) {
-                    const int col = n0 + c + half * 32;
-                    const float ws = col + lane < a.N ? a.ws[col + lane] : 0.0f;              // column `lane`'s; handed round below
-                    unsigned v[32];
-                    tmem_ld_32x32(tmem_row + (unsigned)(c + half * 32), v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (c + COLS >= col0 + BN / 2 && half == COLS / 32 - 1) {                            // its half of the tile has left tensor memory
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(acc_empty_first + (unsigned)(b * 8));
-                    }
+                for (int e = 0; e < 32; ++e) f[e] = __float_as_uint(__uint_as_float(f[e]) * xs * __shfl_sync(0xffffffffu, ws[j], e));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * xs * __shfl_sync(0xffffffffu, ws, j));
-                    if (TMA_STORE) {
-                        // row `lane` of the piece; its 16-byte chunk q goes to position q ^ (lane % 8): the 128-byte swizzle
-                        if (sizeof(O) == 4) {
+                for (int h = 0; h < PIECES; ++h) {
+                    unsigned char* buf = own + (j * PIECES + h & 1) * 2048;
+                    if (TMA_STORE && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");     // the store before the last has read its piece
+                    __syncwarp();
+                    // row `lane` of the piece; its 16-byte chunk q goes to position q ^ (lane / 2 % 4): the 64-byte swizzle
 #pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                        } else {
+                    for (int q = 0; q < 4; ++q) {
+                        unsigned w[4];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                unsigned pw[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
-                                    pw[e] = *reinterpret_cast<const unsigned*>(&h);
-                                }
-                                *reinterpret_cast<uint4*>(buf + lane * 128 + (((half * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+                        for (int e = 0; e < 4; ++e) {
+                            if (PIECES == 2) w[e] = f[h * 16 + 4 * q + e];
+                            else {
+                                const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(f[(8 * q + 2 * e) & 31]), __uint_as_float(f[(8 * q + 2 * e + 1) & 31]));
+                                w[e] = *reinterpret_cast<const unsigned*>(&two);
                             }
                         }
-                    } else if (row < a.M && col < a.N) {
-                        O* dst = reinterpret_cast<O*>(a.out) + (size_t)row * a.ldo + col;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + j < a.N) dst[j] = from_f32<O>(__uint_as_float(v[j]));
+                        *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ swizzle) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                }
-                if (TMA_STORE) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");              // the writes above, seen by the TMA
-                    __syncwarp();
-                    if (lane == 0) {
-                        // rows or columns of the piece that lie outside the matrix are clipped
-                        if (m0 + quarter * 32 < a.M && n0 + c < a.N) tma_store_2d(&map_o, buf, n0 + c, m0 + quarter * 32);
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    const int col = n0 + j * 32 + h * COLS;
+                    if (TMA_STORE) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");          // the writes above, seen by the TMA
+                        __syncwarp();
+                        if (lane == 0) {
+                            // rows or columns of the piece that lie outside the matrix are clipped
+                            if (m0 < a.M && col < a.N) tma_store_2d(&map_o, buf, col, m0);
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    } else {
+                        // an output whose rows begin anywhere: value by value, the lanes along a row
+                        __syncwarp();
+                        const int at = lane % COLS, last = min(32, a.M - m0);
+                        O* to = reinterpret_cast<O*>(a.out) + (long long)(m0 + lane / COLS) * a.ldo + col + at;
+                        if (col + at < a.N)
+#pragma unroll 8
+                            for (int r = lane / COLS; r < last; r += PIECES, to += PIECES * a.ldo)
+                                *to = *reinterpret_cast<const O*>(buf + r * 64 + ((((at * (int)sizeof(O)) >> 4) ^ ((r >> 1) & 3)) << 4) + ((at * (int)sizeof(O)) & 15));
                     }
                 }
             }
@@ -244,8 +248,8 @@ int launch(const Args& a, cudaStream_t s) {
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, a.K, a.ldx, BM, STEP)) return rc;
     if (int rc = make_map(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, a.K, a.ldw, BN / 2, STEP)) return rc;
     if ((uintptr_t)a.out % 16 == 0 && a.ldo * (long long)sizeof(O) % 16 == 0) {
-        if (int rc = make_map(&mo, a.out, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (int)sizeof(O), a.M, a.N, a.ldo, 32,
-                              128 / (int)sizeof(O))) return rc;
+        if (int rc = wide::make_map_swizzled(&mo, a.out, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (int)sizeof(O), a.M, a.N, a.ldo,
+                                             32, 64 / (int)sizeof(O), CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
         return launch_kernel<O, true>(mx, mw, mo, a, s);
     }
     mo = mx;

@@ -35,10 +35,6 @@ struct Barriers {
     int abort_flag;
 };
 
-// An arrival at the first block's barrier (`bar`: an address in the cluster's shared window) that passes on nothing but tensor memory, which
-// tcgen05.wait and tcgen05.fence order: released to the cluster (mbar_arrive_cluster) it would wait for all of the thread's loads and stores
-// first, some 1,500 cycles in every step.
-__device__ __forceinline__ void mbar_arrive_first(unsigned bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A step's eight instructions, 16 values each: the weights' columns follow one another, the tokens' tile has 32 bytes more each, and its second
 // half, 64 values on, is a tile of its own.  In one piece, so that little stands between them: the warp that issues shares its scheduler with
 // four others, and a step is 768 cycles.
@@ -205,7 +201,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_first(ready_first + (unsigned)(place * 8));
+                if (lane == 0) wide::mbar_arrive_remote(ready_first + (unsigned)(place * 8));
             }
         }
     } else {
@@ -226,7 +222,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                 if (j + 16 >= nt) {                                                   // all of it is in registers: the accumulator may be filled again
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_first(acc_empty_first + (unsigned)(b * 8));
+                    if (lane == 0) wide::mbar_arrive_remote(acc_empty_first + (unsigned)(b * 8));
                 }
                 if (n < g.N)
 #pragma unroll

@@ -66,6 +66,10 @@ __device__ __forceinline__ void tmem_load8(unsigned addr, unsigned (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(addr));
 }
+// An arrival at another block's barrier (`bar`: an address in the cluster's shared window) that passes on nothing but tensor memory, which
+// tcgen05.wait and tcgen05.fence order: released to the cluster (mbar_arrive_cluster) it would wait for all of the thread's loads and stores
+// first, some 1,500 cycles.
+__device__ __forceinline__ void mbar_arrive_remote(unsigned bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A request to bring a box into L2: it holds nothing back and may come ahead of what is written there.
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
