@@ -198,6 +198,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 #pragma unroll 8
                             for (int r = lane / COLS; r < last; r += PIECES, to += PIECES * a.ldo)
                                 *to = *reinterpret_cast<const O*>(buf + r * 64 + ((((at * (int)sizeof(O)) >> 4) ^ ((r >> 1) & 3)) << 4) + ((at * (int)sizeof(O)) & 15));
+                        __syncwarp();
                     }
                 }
             }

@@ -10,7 +10,8 @@
 //   * twelve warps, in three sets that take the steps in turn, make bfloat16 numbers s (c - z) of the codes, a weight row a lane, in the block's
 //     tensor memory, and say so to the first block, where one warp issues the instructions for both (256 x NT x 16).  (A set needs 2,100
 //     cycles from step to step, a third of them waits and messages: two sets were slower than the instructions, which take 768 at 192 tokens);
-//   * four warps read the block's half of the accumulator, which is double-buffered, and store it.
+//   * four warps read the block's half of the accumulator, which is double-buffered, and store it, a token's 32 neighbouring values at a time
+//     (through shared memory and TMA: 1900 x 7168 x 5120 94.0 us, as it is 94.9; 1999 x 8192 x 256 25.2, 23.3).
 // The accumulators take 2 NT columns of tensor memory and the weights the rest, 64 columns a step: NT is at most 192.
 // All waits are bounded (umma.cuh).
 #pragma once
@@ -67,7 +68,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
     const unsigned rank = cluster_rank();                                             // 0: the block that issues the pair's instructions
     const int steps = (g.K + STEP - 1) / STEP, m_tiles = (g.M + nt - 1) / nt, n_tiles = (g.N + TILE_N - 1) / TILE_N;
-    const long long tiles = (long long)m_tiles * n_tiles;
+    const int tiles = m_tiles * n_tiles;                                              // (16,384 outputs each at least: fewer than 2^31 in any memory)
     const int walker = (int)(blockIdx.x >> 1), walkers = (int)(gridDim.x >> 1);
 
     if (threadIdx.x == 0) {
@@ -99,8 +100,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         wide::Ring at(stages);
         unsigned it = 0;
         bool ok = true;
-        for (long long t = walker; t < tiles && ok; t += walkers) {
-            const int m0 = (int)(t % m_tiles) * nt + (int)rank * (nt / 2), n0 = (int)(t / m_tiles) * TILE_N + (int)rank * BM;
+        for (int t = walker; t < tiles && ok; t += walkers) {
+            const int m0 = t % m_tiles * nt + (int)rank * (nt / 2), n0 = t / m_tiles * TILE_N + (int)rank * BM;
             for (int c = 0; c < steps; ++c, ++it, at.next()) {
                 const int s = at.stage;
                 ok = mbar_wait(&bar->done[s], at.phase ^ 1, abort_flag, 21) && !*abort_flag;
@@ -129,7 +130,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             wide::Ring at(stages), made(g.w_stages);
             bool ok = true;
             int i = 0;
-            for (long long t = walker; t < tiles && ok; t += walkers, ++i) {
+            for (int t = walker; t < tiles && ok; t += walkers, ++i) {
                 const int b = i & 1;
                 ok = mbar_wait(&bar->acc_empty[b], ((i >> 1) & 1) ^ 1, abort_flag, 24);      // this accumulator has been read
                 if (!ok) break;
@@ -164,70 +165,91 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             if (stage >= stages) { stage -= stages; phase ^= 1; }
             place = (place + SETS) % g.w_stages;
         };
-        int c = set;                                                                  // the step inside its tile
-        for (long long t = walker; t < tiles && ok; t += walkers, c -= steps) {
-            const long long weight_row = min((int)(t / m_tiles) * TILE_N + (int)rank * BM + row, g.N - 1);
-            const bf16* scales = g.scales + weight_row * g.lds;
-            const unsigned char* zeros = ZEROS ? g.zeros + weight_row * g.lds : nullptr;
-            wide::Group<RUNS, ZEROS> ahead;
-            if (c < steps) ahead.fetch(scales, zeros, c, groups);
-            for (; c < steps; c += SETS, next()) {
-                const int s = stage;
-                const wide::Group<RUNS, ZEROS> now = ahead;
-                ahead.fetch(scales, zeros, c + SETS, groups);
-                ok = mbar_wait(&bar->w_full[s], phase, abort_flag, 25);
-                if (!ok) break;
-                // unit q holds word 4 q + j; the 64-byte swizzle put it at q ^ (row / 2 % 4), so that eight lanes meet no bank twice
-                const unsigned char* src = w_tiles + s * W_BYTES + row * 64;
-                unsigned words[4][4], v[4][16];
+        // the set's next step is step c of tile t: its scales are on their way before the step's codes are looked at, over the end of a tile too
+        int c = set, t = walker;
+        const bf16* scales = nullptr;
+        const unsigned char* zeros = nullptr;
+        auto locate = [&] {
+            for (; c >= steps; c -= steps) t += walkers;
+            const long long weight_row = min(t / m_tiles * TILE_N + (int)rank * BM + row, g.N - 1);
+            scales = g.scales + weight_row * g.lds;
+            if (ZEROS) zeros = g.zeros + weight_row * g.lds;
+        };
+        locate();
+        wide::Group<RUNS, ZEROS> ahead;
+        if (t < tiles) ahead.fetch(scales, zeros, c, groups);
+        while (t < tiles) {
+            const int s = stage;
+            const wide::Group<RUNS, ZEROS> now = ahead;
+            c += SETS;
+            if (c >= steps) locate();
+            if (t < tiles) ahead.fetch(scales, zeros, c, groups);
+            ok = mbar_wait(&bar->w_full[s], phase, abort_flag, 25);
+            if (!ok) break;
+            // unit q holds word 4 q + j; the 64-byte swizzle put it at q ^ (row / 2 % 4), so that eight lanes meet no bank twice
+            const unsigned char* src = w_tiles + s * W_BYTES + row * 64;
+            unsigned words[4][4], v[4][16];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(words[q]) = *reinterpret_cast<const uint4*>(src + ((q ^ ((row >> 1) & 3)) << 4));
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(words[q]) = *reinterpret_cast<const uint4*>(src + ((q ^ ((row >> 1) & 3)) << 4));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) now.numbers(words[q][j], j / RUNS, v[j] + q * 4);
-                // (the numbers wait in registers for their place, of which there are few: from one step's end to the next one's beginning in a
-                // place only the way into tensor memory and the messages take time)
-                if (!first) {
-                    const int before = stage - g.w_stages;
-                    ok = mbar_wait(&bar->done[before < 0 ? before + stages : before], before < 0 ? phase ^ 1 : phase, abort_flag, 26);
-                }
-                // (one warp also sees that the tokens' rows are there, for the warp that issues: a wait takes that one some 300 cycles of a step)
-                if (ok && rank == 0 && quarter == 0) ok = mbar_wait(&bar->x_full[s], phase, abort_flag, 22);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int j = 0; j < 4; ++j) wide::tmem_store16(mine + (unsigned)(place * 64 + j * 16), v[j]);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) wide::mbar_arrive_remote(ready_first + (unsigned)(place * 8));
+                for (int q = 0; q < 4; ++q) now.numbers(words[q][j], j / RUNS, v[j] + q * 4);
+            // (the numbers wait in registers for their place, of which there are few: from one step's end to the next one's beginning in a
+            // place only the way into tensor memory and the messages take time)
+            if (!first) {
+                const int before = stage - g.w_stages;
+                ok = mbar_wait(&bar->done[before < 0 ? before + stages : before], before < 0 ? phase ^ 1 : phase, abort_flag, 26);
             }
+            // (one warp also sees that the tokens' rows are there, for the warp that issues: a wait takes that one some 300 cycles of a step)
+            if (ok && rank == 0 && quarter == 0) ok = mbar_wait(&bar->x_full[s], phase, abort_flag, 22);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wide::tmem_store16(mine + (unsigned)(place * 64 + j * 16), v[j]);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) wide::mbar_arrive_remote(ready_first + (unsigned)(place * 8));
+            next();
         }
     } else {
         // ------------------------------------------------------------------ the way out: a warp for every 32 weight rows
         const unsigned acc_empty_first = map_to_cta(smem_u32(&bar->acc_empty[0]), 0);
         int i = 0;
-        for (long long t = walker; t < tiles; t += walkers, ++i) {
-            const int m0 = (int)(t % m_tiles) * nt, n = (int)(t / m_tiles) * TILE_N + (int)rank * BM + quarter * 32 + lane, b = i & 1;
+        for (int t = walker; t < tiles; t += walkers, ++i) {
+            const int m0 = t % m_tiles * nt, n = t / m_tiles * TILE_N + (int)rank * BM + quarter * 32 + lane, b = i & 1;
             if (!mbar_wait(&bar->acc_full[b], (i >> 1) & 1, abort_flag, 27)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned mine = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(b * nt);
-            bf16* out = g.out + (long long)m0 * g.ldo + n;
-            for (int j = 0; j < nt; j += 16) {
-                unsigned v[2][8];
-                wide::tmem_load8(mine + (unsigned)j, v[0]);
-                wide::tmem_load8(mine + (unsigned)j + 8, v[1]);
+            // 32 tokens' values of this lane's weight row
+            auto put = [&](const unsigned (&v)[32], int j) {
+                if (n >= g.N) return;
+                const int left = g.M - m0 - j;
+                bf16* to = g.out + (long long)(m0 + j) * g.ldo + n;
+#pragma unroll
+                for (int e = 0; e < 32; ++e, to += g.ldo)
+                    if (e < left) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+            };
+            // the next values are on their way out of tensor memory while these are stored; behind the last the accumulator may be filled again
+            auto next = [&](unsigned (&v)[32], int j) {
+                __syncwarp();
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (j + 16 >= nt) {                                                   // all of it is in registers: the accumulator may be filled again
+                if (j < nt) tmem_ld_32x32(mine + (unsigned)j, v);
+                else {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) wide::mbar_arrive_remote(acc_empty_first + (unsigned)(b * 8));
                 }
-                if (n < g.N)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (m0 + j + e < g.M) out[(long long)(j + e) * g.ldo] = __float2bfloat16_rn(__uint_as_float(v[e >> 3][e & 7]));
+            };
+            unsigned v0[32], v1[32];
+            tmem_ld_32x32(mine, v0);
+            for (int j = 0; j < nt; j += 64) {
+                next(v1, j + 32);
+                put(v0, j);
+                if (j + 32 >= nt) break;
+                next(v0, j + 64);
+                put(v1, j + 32);
             }
         }
     }
@@ -264,7 +286,8 @@ int pairs_held() {
 }
 
 // The tile width that takes the fewest cycles, and how many: a step takes 780 and 1.6 for every token of the tile (1900 x 7168 x 5120, tiles of 64 /
-// 128 / 160 / 192: 226 / 124 / 113 / 98 us).
+// 128 / 160 / 192: 226 / 124 / 113 / 98 us), the way from one tile to the next 2,400, and a tile at least 36 for every token, which its way out takes
+// (96 / 768 x 24576 x 256: 7.6 / 25.2 us).
 template <int RUNS, bool ZEROS>
 int shape(PairArgs& g, double* cycles) {
     static LlmeGrants grants;
@@ -273,7 +296,9 @@ int shape(PairArgs& g, double* cycles) {
     *cycles = -1.0;
     for (int nt = 64; nt <= MOST_NT; nt += 32) {
         const long long tiles = (long long)n_tiles * ((g.M + nt - 1) / nt);
-        const double cost = (double)((tiles + held - 1) / held) * ((g.K + STEP - 1) / STEP) * (780.0 + 1.6 * nt) + 11000.0;
+        double tile = ((g.K + STEP - 1) / STEP) * (780.0 + 1.6 * nt) + 2400.0;
+        if (tile < 36.0 * nt) tile = 36.0 * nt;
+        const double cost = (double)((tiles + held - 1) / held) * tile + 5000.0;
         if (*cycles < 0.0 || cost < *cycles) { *cycles = cost; g.nt = nt; }
     }
     g.w_stages = (512 - 2 * g.nt) / 64 < MOST_STAGES ? (512 - 2 * g.nt) / 64 : MOST_STAGES;

@@ -234,23 +234,58 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     float* part = reinterpret_cast<float*>(smem);                  // [token][128 weight rows]
     if (warp < WORKERS) {
         const int row = quarter * 32 + lane, n = n0 + row, half = nt / 2, col0 = (warp >> 2) * half;
+        const int first = m0 + col0, left = n < g.N ? min(half, g.M - first) : 0;       // the half's first token; how many of its values are stored
+        // (the scales are there before the sums are: token 32 i + lane's, handed round below)
+        const float ws = !INT4 && g.segments == 1 && n < g.N ? g.ws[n] : 1.0f;
+        float xs[4];
+        if (!INT4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xs[i] = g.segments == 1 && 32 * i + lane < half && first + 32 * i + lane < g.M ? g.xs[first + 32 * i + lane] : 0.0f;
         const bool sum = mbar_wait(&bar->acc, 0, abort_flag, 5);
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned mine = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)col0;
-        const float ws = !INT4 && g.segments == 1 && n < g.N ? g.ws[n] : 1.0f;
-        for (int j = 0; sum && j < half; j += 8) {
-            unsigned v[8];
-            tmem_load8(mine + (unsigned)j, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        auto put = [&](const unsigned (&v)[8], int j) {
+            float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int m = m0 + col0 + j + e;
-                float f = __uint_as_float(v[e]);
-                if (g.segments > 1) part[(col0 + j + e) * BM + row] = f;
-                else if (m < g.M && n < g.N) {
-                    if (!INT4) f = f * g.xs[m] * ws;
-                    store_value(g, m, n, f);
-                }
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[e]);
+            if (g.segments > 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) part[(col0 + j + e) * BM + row] = f[e];
+                return;
+            }
+            if (!INT4) {
+                const float scales = j < 32 ? xs[0] : (j < 64 ? xs[1] : (j < 96 ? xs[2] : xs[3]));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = f[e] * __shfl_sync(0xffffffffu, scales, (j & 31) + e) * ws;
+            }
+            if (!INT4 && g.out_f32) {
+                float* to = reinterpret_cast<float*>(g.out) + (long long)(first + j) * g.ldo + n;
+#pragma unroll
+                for (int e = 0; e < 8; ++e, to += g.ldo)
+                    if (j + e < left) *to = f[e];
+            } else {
+                bf16* to = reinterpret_cast<bf16*>(g.out) + (long long)(first + j) * g.ldo + n;
+#pragma unroll
+                for (int e = 0; e < 8; ++e, to += g.ldo)
+                    if (j + e < left) *to = __float2bfloat16_rn(f[e]);
+            }
+        };
+        // the next values are on their way out of tensor memory while these are stored
+        auto next = [&](unsigned (&v)[8], int j) {
+            __syncwarp();
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (j < half) tmem_load8(mine + (unsigned)j, v);
+        };
+        if (sum) {
+            unsigned v0[8], v1[8];
+            tmem_load8(mine, v0);
+            for (int j = 0; j < half; j += 16) {
+                next(v1, j + 8);
+                put(v0, j);
+                if (j + 8 >= half) break;
+                next(v0, j + 16);
+                put(v1, j + 8);
             }
         }
     }
@@ -347,7 +382,8 @@ int clusters_held(int segments, int per_sm) {
 
 // Tile width, segments, blocks an SM and stages of a product: what a model of its time says is least, in cycles.  The blocks that run at once
 // (as many as are held) share the memory's 2,900 bytes a cycle for the weights; an SM's blocks share its 42 bytes a cycle from L2 and its
-// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16).  Starting and ending a block cost about 5,000
+// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16), and making numbers of a step's codes keeps an SM busy
+// for 1,050.  Starting and ending a block cost about 5,000
 // cycles and 14 for every token, the cluster's sums 1,000 and 16.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
 // 19.2 us, both in segments of four.)
 template <bool INT4, int RUNS, bool ZEROS>
@@ -368,6 +404,7 @@ int shape(Args& g, double* cycles) {
                 const double rounds = (double)((tiles + held - 1) / held), at_once = (double)(tiles < held ? tiles : held) * segments;
                 const double share = at_once > sm_count() ? at_once / sm_count() : 1.0;                   // blocks on an SM
                 double step = share * (INT4 ? 4.0 : 2.0) * nt;
+                if (INT4 && step < 1050.0 * (at_once > sm_count() ? 2.0 : 1.0)) step = 1050.0 * (at_once > sm_count() ? 2.0 : 1.0);
                 if (step < share * (w_bytes + nt * x_width) / 42.0) step = share * (w_bytes + nt * x_width) / 42.0;
                 if (step < at_once * w_bytes / 2900.0) step = at_once * w_bytes / 2900.0;
                 const double cost = rounds * (each * step + 5000.0 + 14.0 * nt + (segments > 1 ? 1000.0 + 16.0 * nt : 0.0));
