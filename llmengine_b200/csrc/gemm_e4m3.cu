@@ -133,8 +133,9 @@ int launch_skinny(const Args& a, cudaStream_t s) {
 }
 
 // More tokens than the weight-streaming kernel takes at once: 256 x 256 tiles on pairs of SMs, or narrower tiles with K cut over a cluster,
-// whichever a model of its time says is faster.  A step of 128 values takes a pair 580 cycles, a tile 4,300 at least, which its way out takes,
-// and starting and the last tile some 7,500 (384 x 4096 x 512 / 4096: 5.5 / 14.2 us, 2048 x 24576 x 128 29.2).
+// whichever a model of its time says is faster.  A step of 128 values takes a pair 580 cycles, all tiles but the last 4,300 at least, which
+// the way out of the one before takes, and starting and the last one's way out some 9,800 (384 x 4096 x 512 / 4096: 5.4 / 14.2 us, 2048 x 24576 x
+// 128 29.2).
 template <typename O>
 int launch_wide(const Args& a, cudaStream_t s) {
     constexpr int out_f32 = sizeof(O) == 4;
@@ -147,7 +148,7 @@ int launch_wide(const Args& a, cudaStream_t s) {
     if (int rc = wide::shape<false, 4, false>(g, &cycles)) return rc;
     const long long pairs = sm_count() / 2, tiles = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
     const double tile = (a.K + 127) / 128 * 580.0;
-    const double paired = (double)((tiles + pairs - 1) / pairs) * (tile < 4300.0 ? 4300.0 : tile) + 7500.0;
+    const double paired = (double)((tiles + pairs - 1) / pairs - 1) * (tile < 4300.0 ? 4300.0 : tile) + tile + 9800.0;
     if (g_form == 2 || (g_form == 0 && paired < cycles)) return pair::launch<O>(a, s);
     alignas(64) CUtensorMap mw, mx;
     if (int rc = make_map(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, a.K, a.ldw, BM, wide::STEP)) return rc;

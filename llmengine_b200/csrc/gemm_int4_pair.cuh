@@ -11,7 +11,7 @@
 //     tensor memory, and say so to the first block, where one warp issues the instructions for both (256 x NT x 16).  (A set needs 2,100
 //     cycles from step to step, a third of them waits and messages: two sets were slower than the instructions, which take 768 at 192 tokens);
 //   * four warps read the block's half of the accumulator, which is double-buffered, and store it, a token's 32 neighbouring values at a time
-//     (through shared memory and TMA: 1900 x 7168 x 5120 94.0 us, as it is 94.9; 1999 x 8192 x 256 25.2, 23.3).
+//     (1999 x 8192 x 256, little else: 17 us; through shared memory and TMA 25).
 // The accumulators take 2 NT columns of tensor memory and the weights the rest, 64 columns a step: NT is at most 192.
 // All waits are bounded (umma.cuh).
 #pragma once
@@ -222,14 +222,19 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             if (!mbar_wait(&bar->acc_full[b], (i >> 1) & 1, abort_flag, 27)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned mine = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(b * nt);
-            // 32 tokens' values of this lane's weight row
+            // 32 tokens' values of this lane's weight row (all of them wherever there are so many: a test at every store took twice as long)
             auto put = [&](const unsigned (&v)[32], int j) {
                 if (n >= g.N) return;
                 const int left = g.M - m0 - j;
                 bf16* to = g.out + (long long)(m0 + j) * g.ldo + n;
+                if (left >= 32) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e, to += g.ldo)
-                    if (e < left) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+                    for (int e = 0; e < 32; ++e, to += g.ldo) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e, to += g.ldo)
+                        if (e < left) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+                }
             };
             // the next values are on their way out of tensor memory while these are stored; behind the last the accumulator may be filled again
             auto next = [&](unsigned (&v)[32], int j) {
@@ -285,9 +290,10 @@ int pairs_held() {
     return n;
 }
 
-// The tile width that takes the fewest cycles, and how many: a step takes 780 and 1.6 for every token of the tile (1900 x 7168 x 5120, tiles of 64 /
-// 128 / 160 / 192: 226 / 124 / 113 / 98 us), the way from one tile to the next 2,400, and a tile at least 36 for every token, which its way out takes
-// (96 / 768 x 24576 x 256: 7.6 / 25.2 us).
+// The tile width that takes the fewest cycles, and how many: a step takes 780 and one for every token of the tile (1900 x 7168 x 5120, tiles of 64 /
+// 128 / 160 / 192: 226 / 124 / 113 / 92 us), the way from one tile to the next 1,500; all tiles but the last take 4,000 and three for every token at
+// least, which the way out of the one before takes (768 / 1600 x 24576 x 256: 17.8 / 32.7 us); starting takes 3,300, the last one's way out 23 for
+// every token.
 template <int RUNS, bool ZEROS>
 int shape(PairArgs& g, double* cycles) {
     static LlmeGrants grants;
@@ -296,9 +302,8 @@ int shape(PairArgs& g, double* cycles) {
     *cycles = -1.0;
     for (int nt = 64; nt <= MOST_NT; nt += 32) {
         const long long tiles = (long long)n_tiles * ((g.M + nt - 1) / nt);
-        double tile = ((g.K + STEP - 1) / STEP) * (780.0 + 1.6 * nt) + 2400.0;
-        if (tile < 36.0 * nt) tile = 36.0 * nt;
-        const double cost = (double)((tiles + held - 1) / held) * tile + 5000.0;
+        const double tile = ((g.K + STEP - 1) / STEP) * (780.0 + nt) + 1500.0, out = 4000.0 + 3.0 * nt;
+        const double cost = (double)((tiles + held - 1) / held - 1) * (tile > out ? tile : out) + tile + 3300.0 + 23.0 * nt;
         if (*cycles < 0.0 || cost < *cycles) { *cycles = cost; g.nt = nt; }
     }
     g.w_stages = (512 - 2 * g.nt) / 64 < MOST_STAGES ? (512 - 2 * g.nt) / 64 : MOST_STAGES;

@@ -74,6 +74,13 @@ __device__ __forceinline__ void mbar_arrive_remote(unsigned bar) { asm volatile(
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
+// Eight tokens' values of a weight row, of which `left` are there.
+template <typename O>
+__device__ __forceinline__ void store8(O* to, long long ldo, int left, const float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e, to += ldo)
+        if (e < left) *to = from_f32<O>(f[e]);
+}
 __device__ __forceinline__ void store_value(const Args& g, long long m, int n, float v) {
     if (g.out_f32) reinterpret_cast<float*>(g.out)[m * g.ldo + n] = v;
     else reinterpret_cast<bf16*>(g.out)[m * g.ldo + n] = __float2bfloat16_rn(v);
@@ -260,15 +267,9 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                 for (int e = 0; e < 8; ++e) f[e] = f[e] * __shfl_sync(0xffffffffu, scales, (j & 31) + e) * ws;
             }
             if (!INT4 && g.out_f32) {
-                float* to = reinterpret_cast<float*>(g.out) + (long long)(first + j) * g.ldo + n;
-#pragma unroll
-                for (int e = 0; e < 8; ++e, to += g.ldo)
-                    if (j + e < left) *to = f[e];
+                store8(reinterpret_cast<float*>(g.out) + (long long)(first + j) * g.ldo + n, g.ldo, left - j, f);
             } else {
-                bf16* to = reinterpret_cast<bf16*>(g.out) + (long long)(first + j) * g.ldo + n;
-#pragma unroll
-                for (int e = 0; e < 8; ++e, to += g.ldo)
-                    if (j + e < left) *to = __float2bfloat16_rn(f[e]);
+                store8(reinterpret_cast<bf16*>(g.out) + (long long)(first + j) * g.ldo + n, g.ldo, left - j, f);
             }
         };
         // the next values are on their way out of tensor memory while these are stored
@@ -381,11 +382,12 @@ int clusters_held(int segments, int per_sm) {
 }
 
 // Tile width, segments, blocks an SM and stages of a product: what a model of its time says is least, in cycles.  The blocks that run at once
-// (as many as are held) share the memory's 2,900 bytes a cycle for the weights; an SM's blocks share its 42 bytes a cycle from L2 and its
-// tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16), and making numbers of a step's codes keeps an SM busy
-// for 1,050.  Starting and ending a block cost about 5,000
-// cycles and 14 for every token, the cluster's sums 1,000 and 16.  (Measured: 8 bits, 20 x 4096 x 512 / 12288 3.4 / 12.6 us, 256 x 4096 x 12288
-// 19.2 us, both in segments of four.)
+// (as many as are held) share the memory's 4,000 bytes a cycle for the weights; an SM's blocks share its 60 bytes a cycle from L2 (52 beside the
+// making of numbers) and its tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16); making numbers of a step's
+// codes keeps an SM busy for 850.  Starting and ending a block cost about 4,000 cycles and 22 for every token, the cluster's sums 3,000 and 10.
+// Over 42 products of 40 to 1,600 tokens and all of their tilings the model is off by 12 % (standard deviation), and its choice took 1 % longer than
+// the best with 8 bits, 2 % with 4.  (200 x 4096 x 4096 in 8 bits, tiles of 208 tokens in four segments, 10.7 us; 96 x 7168 x 5120 in 4 bits, two
+// segments, 15.6, where tiles of 48, two blocks an SM, take 31.)
 template <bool INT4, int RUNS, bool ZEROS>
 int shape(Args& g, double* cycles) {
     const int steps = (g.K + STEP - 1) / STEP, n_tiles = (g.N + BM - 1) / BM, w_bytes = INT4 ? BM * STEP / 2 : BM * STEP, x_width = STEP * (INT4 ? 2 : 1);
@@ -404,10 +406,10 @@ int shape(Args& g, double* cycles) {
                 const double rounds = (double)((tiles + held - 1) / held), at_once = (double)(tiles < held ? tiles : held) * segments;
                 const double share = at_once > sm_count() ? at_once / sm_count() : 1.0;                   // blocks on an SM
                 double step = share * (INT4 ? 4.0 : 2.0) * nt;
-                if (INT4 && step < 1050.0 * (at_once > sm_count() ? 2.0 : 1.0)) step = 1050.0 * (at_once > sm_count() ? 2.0 : 1.0);
-                if (step < share * (w_bytes + nt * x_width) / 42.0) step = share * (w_bytes + nt * x_width) / 42.0;
-                if (step < at_once * w_bytes / 2900.0) step = at_once * w_bytes / 2900.0;
-                const double cost = rounds * (each * step + 5000.0 + 14.0 * nt + (segments > 1 ? 1000.0 + 16.0 * nt : 0.0));
+                if (INT4 && step < 850.0 * (at_once > sm_count() ? 2.0 : 1.0)) step = 850.0 * (at_once > sm_count() ? 2.0 : 1.0);
+                if (step < share * (w_bytes + nt * x_width) / (INT4 ? 52.0 : 60.0)) step = share * (w_bytes + nt * x_width) / (INT4 ? 52.0 : 60.0);
+                if (step < at_once * w_bytes / 4000.0) step = at_once * w_bytes / 4000.0;
+                const double cost = rounds * (each * step + 4000.0 + 22.0 * nt + (segments > 1 ? 3000.0 + 10.0 * nt : 0.0));
                 if (best < 0.0 || cost < best) { best = cost; g.nt = nt; g.segments = segments; g.segment_steps = each; g.per_sm = per_sm; }
             }
     }
