@@ -5,11 +5,14 @@
 // sixteen 32-bit words holds values 32 j + 8 q .. + 7, the even ones in the low half, the odd ones in the high half, four bits each, in
 // order.  So lane q of a quad finds in ONE 16-byte load eight values of each of the block's four runs of 32: the 16 values of a matrix
 // instruction always lie in one group, whichever G.  And (word >> 4 p) & 0x000f000f are the codes of two neighbouring values in the two
-// halves of a register: with 0x4300 in front of each they are the bfloat16 numbers 128 + c, from which 128 + z is subtracted exactly.
+// halves of a register, from where one or two instructions make two bfloat16 numbers of them (eight_codes(), wide::Group).
 //
-// A handful of tokens: bound by reading the codes.  As in the bfloat16 product (gemm_skinny.cu) 16 weight rows are the M side of a
-// mma.sync.m16n8k16 tile and the tokens its N side.  The codes c - z enter the instruction as they are; a group's sums are multiplied by
-// its scale, in 32-bit, when the group ends: no weight is rounded.
+// Up to 16 tokens: bound by reading the codes.  As in the bfloat16 product (gemm_skinny.cu) 16 weight rows are the M side of a
+// mma.sync.m16n8k16 tile and the tokens its N side; the codes come through a ring in shared memory (weight_stream.cuh).  They enter the
+// instruction as (c - z) 2^-6; a group's sums are multiplied by its scale, in 32-bit, when the group ends: no weight is rounded.
+// 1 x 24576 x 4096, groups of 128: 13.8 us, 3.8 TB/s, where the loads alone take 10.1: what is left is making numbers of the codes, on which
+// the cores work between half and two thirds of the time.  A group of 32 has four times the scales: 1 x 4096 x 4096 4.4 us, 5.5.
+// More: tcgen05, the weights made into bfloat16 numbers in tensor memory, on single SMs (gemm_wide.cuh) or on pairs (gemm_int4_pair.cuh).
 //
 // The reference's weight-only product has 8-bit blocks (src/runtime/kernels/cuda_kernels.cu:296-358); it has none of 4 bits.
 #include <cuda.h>
@@ -199,13 +202,12 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
         for (int i = 0; i < 4; ++i) acc[m][i] *= 64.0f;                            // (the codes were numbers of 2^-6)
     // the sums of the warps that share a row group, added in their order
     float (*red)[16] = reinterpret_cast<float (*)[16]>(rings);                     // [warp * 8 MT + token][row]: over the rings, which are empty now
-    if (SHARE > 1) __syncthreads();
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) red[warp * MT * 8 + m * 8 + quad * 2 + (i & 1)][r + (i >> 1) * 8] = acc[m][i];
-    if (SHARE > 1) __syncthreads();
-    else __syncwarp();
+    __syncthreads();
     for (int i = part * 32 + lane; i < MT * 8 * 16; i += SHARE * 32) {
         const int tok = i >> 4, row = n0 + (i & 15);
         if (tok >= a.M || row >= a.N) continue;

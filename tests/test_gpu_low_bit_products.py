@@ -125,6 +125,20 @@ def test_e4m3_rows_that_are_no_numbers(forms, m):
 
 
 # ----------------------------------------------------------------------------- 4 bits
+# Many tiles for every pair of SMs and few steps in each: the ends of tiles in every order that the steps can have.
+MANY_TILES = [(1000, 9000), (777, 12289)]
+
+
+@pytest.mark.parametrize("m,n", MANY_TILES)
+@pytest.mark.parametrize("k", [16, 256, 272, 640])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_e4m3_many_tiles(forms, m, n, k, dtype):
+    x, xs, w, ws = _whole_e4m3(m, n, k, seed=m + k)
+    whole, out = _out(m, n, dtype, 0)
+    forms.linear_e4m3(x, xs, w, ws, out)
+    assert torch.equal(out, _exact_e4m3(x, xs, w, ws).to(dtype))
+
+
 def _whole_int4(m, n, k, group, zeros, seed):
     """Whole numbers -4..4, any codes, scales 2^-3..2^3, zero points over the whole range: |sum| <= 4 * 15 * 2^3 k in steps of 2^-3: exact in 32
     bits for k < 2^15."""
@@ -154,6 +168,17 @@ def test_int4_places(forms, m, n, k, group, zeros):
         assert forms.linear_int4(x, pack_int4(codes), scales, out, zeros=zero) is out
         assert torch.equal(out, want)
         _rest_untouched(whole, n)
+
+
+@pytest.mark.parametrize("m,n", MANY_TILES)
+@pytest.mark.parametrize("k", [40, 200, 384, 520, 1032])
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+def test_int4_many_tiles(forms, m, n, k, group, zeros):
+    from llmengine_b200.weights.quantize import pack_int4
+    x, codes, scales, zero = _whole_int4(m, n, k, group, zeros, seed=m + k)
+    whole, out = _out(m, n, torch.bfloat16, 0)
+    forms.linear_int4(x, pack_int4(codes), scales, out, zeros=zero)
+    assert torch.equal(out, (x.double() @ _weights64(codes, scales, zero, group).t()).to(torch.bfloat16))
 
 
 @pytest.mark.parametrize("m", [1, 8, 16, 40, 77, 128, 300, 1024])
