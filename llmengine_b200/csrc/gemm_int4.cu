@@ -40,7 +40,7 @@ struct Args {
     const bf16* scales; const unsigned char* zeros; long long lds;      // values from row to row of both
     bf16* out; long long ldo;
     int M, N, K;
-    int vec_scales;                                         // a block's scales and zero points begin on their size
+    int together;                                           // scales and zero points that lie on their size: 2 a piece's, 1 a block's, 0 one
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -61,51 +61,63 @@ __device__ __forceinline__ void eight_codes(unsigned word, __nv_bfloat162 minus_
         v[p] = *reinterpret_cast<const unsigned*>(&w);
     }
 }
-// -z 2^-6, twice
-__device__ __forceinline__ __nv_bfloat162 minus_zero_point(unsigned z) { return __float2bfloat162_rn(-(float)z * 0.015625f); }
-
-// COUNT neighbouring scales (2 bytes each) or zero points (1 byte each) side by side in T, in one load where `whole` says that they begin on
-// their size.
-template <typename T, int COUNT, int BYTES>
-__device__ __forceinline__ T load_few(const unsigned char* p, bool whole) {
-    if (COUNT > 1 && whole) {
-        if constexpr (COUNT * BYTES == 2) return *reinterpret_cast<const unsigned short*>(p);
-        else if constexpr (COUNT * BYTES == 4) return *reinterpret_cast<const unsigned*>(p);
-        else if constexpr (COUNT * BYTES == 8) return (T)*reinterpret_cast<const unsigned long long*>(p);
-    }
-    T v = 0;
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v |= (T)(BYTES == 1 ? (unsigned)p[i] : (unsigned)*reinterpret_cast<const unsigned short*>(p + 2 * i)) << (8 * BYTES * i);
-    return v;
+// -z 2^-6, twice, of byte i of `z`: as bits of a bfloat16 number z is z 2^-133, and -2^127 of it is exact.
+__device__ __forceinline__ __nv_bfloat162 minus_zero_point(unsigned z, int i) {
+    const unsigned code = __byte_perm(z, 0u, 0x4040u | (unsigned)i * 0x0101u), factor = 0xff00ff00u;
+    return __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&code), *reinterpret_cast<const __nv_bfloat162*>(&factor), __floats2bfloat162_rn(0.0f, 0.0f));
 }
 
-// What goes with two rows' codes: the scales and zero points of a block of 128 values.
-template <int GROUPS, bool ZEROS>
+// BYTES neighbouring bytes, AT at a time.
+template <int BYTES, int AT>
+__device__ __forceinline__ void take(unsigned* to, const unsigned char* p) {
+#pragma unroll
+    for (int i = 0; i < BYTES; i += AT) {
+        if constexpr (AT == 16) *reinterpret_cast<uint4*>(to + i / 4) = *reinterpret_cast<const uint4*>(p + i);
+        else if constexpr (AT == 8) *reinterpret_cast<uint2*>(to + i / 4) = *reinterpret_cast<const uint2*>(p + i);
+        else if constexpr (AT == 4) to[i / 4] = *reinterpret_cast<const unsigned*>(p + i);
+        else if constexpr (AT == 2) to[i / 4] |= (unsigned)*reinterpret_cast<const unsigned short*>(p + i) << (8 * (i % 4));
+        else to[i / 4] |= (unsigned)p[i] << (8 * (i % 4));
+    }
+}
+
+// What goes with two rows' codes: the scales and zero points of a piece of COUNT groups.  (A load for every row brings all of them where they lie
+// on their size: a load meets eight rows, which takes as long whatever it brings of each.)
+template <int COUNT, bool ZEROS>
 struct Factors {
-    typedef std::conditional_t<GROUPS == 4, unsigned long long, unsigned> S;
-    S s0, s1;
-    unsigned z0, z1;
-    __device__ __forceinline__ void fetch(const Args& a, const unsigned char* scales0, const unsigned char* scales1, size_t row0, size_t row1, int first, int groups) {
-        s0 = s1 = 0;                                        // (behind K there are no scales, and what they would multiply is zero)
-        z0 = z1 = 0;
-        if (first + GROUPS <= groups) {
-            s0 = load_few<S, GROUPS, 2>(scales0 + 2 * (size_t)first, a.vec_scales);
-            s1 = load_few<S, GROUPS, 2>(scales1 + 2 * (size_t)first, a.vec_scales);
-            if (ZEROS) {
-                z0 = load_few<unsigned, GROUPS, 1>(a.zeros + row0 * a.lds + first, a.vec_scales);
-                z1 = load_few<unsigned, GROUPS, 1>(a.zeros + row1 * a.lds + first, a.vec_scales);
-            }
-        } else if (GROUPS > 1) {
-            for (int g = 0; g < GROUPS && first + g < groups; ++g) {
-                s0 |= load_few<S, 1, 2>(scales0 + 2 * (size_t)(first + g), false) << (16 * g);
-                s1 |= load_few<S, 1, 2>(scales1 + 2 * (size_t)(first + g), false) << (16 * g);
-                if (ZEROS) {
-                    z0 |= load_few<unsigned, 1, 1>(a.zeros + row0 * a.lds + first + g, false) << (8 * g);
-                    z1 |= load_few<unsigned, 1, 1>(a.zeros + row1 * a.lds + first + g, false) << (8 * g);
-                }
-            }
+    alignas(16) unsigned s[2][COUNT / 2], z[2][(COUNT + 3) / 4];
+    template <int S_AT, int Z_AT>
+    __device__ __forceinline__ void whole(const unsigned char* const (&scales)[2], const unsigned char* const (&zeros)[2], int first) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            take<2 * COUNT, S_AT>(s[r], scales[r] + 2 * (size_t)first);
+            if (ZEROS) take<COUNT, Z_AT>(z[r], zeros[r] + first);
         }
     }
+    __device__ __forceinline__ void fetch(const Args& a, const unsigned char* const (&scales)[2], const unsigned char* const (&zeros)[2], int first, int groups) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (unsigned& v : s[r]) v = 0;
+#pragma unroll
+            for (unsigned& v : z[r]) v = 0;
+        }
+        if (first + COUNT <= groups) {
+            if (a.together == 2) whole<2 * COUNT, COUNT>(scales, zeros, first);
+            else if (COUNT > 2 && a.together == 1) whole<COUNT, COUNT / 2>(scales, zeros, first);
+            else whole<2, 1>(scales, zeros, first);
+        } else {                                            // (behind K there are no scales, and what they would multiply is zero)
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i)
+                if (first + i < groups)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        s[r][i / 2] |= (unsigned)*reinterpret_cast<const unsigned short*>(scales[r] + 2 * (size_t)(first + i)) << (16 * (i % 2));
+                        if (ZEROS) z[r][i / 4] |= (unsigned)zeros[r][first + i] << (8 * (i % 4));
+                    }
+        }
+    }
+    __device__ __forceinline__ float scale(int r, int i) const { return __uint_as_float(i & 1 ? s[r][i / 2] & 0xffff0000u : s[r][i / 2] << 16); }
+    __device__ __forceinline__ __nv_bfloat162 minus_zero(int r, int i) const { return ZEROS ? minus_zero_point(z[r][i / 4], i % 4) : __floats2bfloat162_rn(-0.125f, -0.125f); }
 };
 
 // MT: 8-token tiles.  RUNS: runs of 32 values in a group (1, 2 or 4).  SHARE: warps that share a row group; AN_SM: warps an SM is to hold.
@@ -118,8 +130,8 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
     const size_t row0 = min(n0 + r, a.N - 1), row1 = min(n0 + r + 8, a.N - 1);            // (a row past the end is read, never stored)
     const unsigned char* w0 = a.w + row0 * a.ldw + quad * 16;
     const unsigned char* w1 = a.w + row1 * a.ldw + quad * 16;
-    const unsigned char* scales0 = reinterpret_cast<const unsigned char*>(a.scales + row0 * a.lds);
-    const unsigned char* scales1 = reinterpret_cast<const unsigned char*>(a.scales + row1 * a.lds);
+    const unsigned char* const scales[2] = {reinterpret_cast<const unsigned char*>(a.scales + row0 * a.lds), reinterpret_cast<const unsigned char*>(a.scales + row1 * a.lds)};
+    const unsigned char* const zeros[2] = {ZEROS ? a.zeros + row0 * a.lds : nullptr, ZEROS ? a.zeros + row1 * a.lds : nullptr};
     // (lanes without a token read the first one: a token's sums are its own, and theirs are not stored)
     const bf16* xp[MT];
 #pragma unroll
@@ -144,9 +156,8 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
     };
 #pragma unroll
     for (int i = 0; i < stream::DEPTH - 1; ++i) bring(i);
-    Factors<GROUPS, ZEROS> next[2], now[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) next[b].fetch(a, scales0, scales1, row0, row1, (2 * part + b) * GROUPS, groups);
+    Factors<2 * GROUPS, ZEROS> next, now;
+    next.fetch(a, scales, zeros, 2 * part * GROUPS, groups);
     // a piece's products; `last`: the piece in which K ends
     auto multiply = [&](int slot, int t, auto last) {
         constexpr bool LAST = decltype(last)::value;
@@ -157,8 +168,8 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
             const unsigned word0[4] = {c0.x, c0.y, c0.z, c0.w}, word1[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                const float f0 = __uint_as_float((unsigned)(now[b].s0 >> (16 * g)) << 16), f1 = __uint_as_float((unsigned)(now[b].s1 >> (16 * g)) << 16);
-                const __nv_bfloat162 z0 = minus_zero_point(ZEROS ? (unsigned)(now[b].z0 >> (8 * g)) & 0xffu : 8u), z1 = minus_zero_point(ZEROS ? (unsigned)(now[b].z1 >> (8 * g)) & 0xffu : 8u);
+                const float f0 = now.scale(0, b * GROUPS + g), f1 = now.scale(1, b * GROUPS + g);
+                const __nv_bfloat162 z0 = now.minus_zero(0, b * GROUPS + g), z1 = now.minus_zero(1, b * GROUPS + g);
                 float sum[MT][4] = {};
 #pragma unroll
                 for (int j = g * RUNS; j < (g + 1) * RUNS; ++j) {
@@ -184,11 +195,8 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
     int slot = 0;
     for (int t = part; t < pieces; t += SHARE) {
         bring(slot == 0 ? stream::DEPTH - 1 : slot - 1);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            now[b] = next[b];
-            next[b].fetch(a, scales0, scales1, row0, row1, (2 * (t + SHARE) + b) * GROUPS, groups);
-        }
+        now = next;
+        next.fetch(a, scales, zeros, 2 * (t + SHARE) * GROUPS, groups);
         stream::Ring::wait();
         if ((t + 1) * PAIR <= a.K) multiply(slot, t, std::false_type{});
         else multiply(slot, t, std::true_type{});
@@ -287,8 +295,8 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     if (meets(span(out, M, N, ldo, 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
         LLME_REFUSE("gemm_int4: the output lies over an operand");
     Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K, 0};
-    const int few = 128 / group;                            // scales of a block
-    a.vec_scales = lds % few == 0 && (uintptr_t)scales % (2 * few) == 0 && (uintptr_t)zeros % few == 0;
+    auto aligned = [&](int count) { return lds % count == 0 && (uintptr_t)scales % (2 * count) == 0 && (uintptr_t)zeros % count == 0; };
+    a.together = aligned(256 / group) ? 2 : (aligned(128 / group) ? 1 : 0);
     if (group == 32) return launch<1>(a, stream);
     if (group == 64) return launch<2>(a, stream);
     return launch<4>(a, stream);
