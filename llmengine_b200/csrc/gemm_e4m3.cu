@@ -9,6 +9,7 @@
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
 #include <cuda.h>
+#include <type_traits>
 
 #include "common.cuh"
 #include "operands.cuh"
@@ -126,10 +127,9 @@ int launch_skinny(const Args& a, cudaStream_t s) {
 }
 template <int MT, typename O>
 int launch_skinny(const Args& a, cudaStream_t s) {
-    stream::Shares by = stream::sharing((a.N + 15) / 16, (a.K + KC - 1) / KC, sm_count());
-    if (by.warps == 16) return launch_skinny<MT, O, 16, 16>(a, s);
-    if (by.warps == 8) return by.an_sm == 16 ? launch_skinny<MT, O, 8, 16>(a, s) : launch_skinny<MT, O, 8, 24>(a, s);
-    return by.warps == 4 ? launch_skinny<MT, O, 4, 24>(a, s) : launch_skinny<MT, O, 2, 24>(a, s);
+    return stream::with(stream::sharing((a.N + 15) / 16, (a.K + KC - 1) / KC, sm_count()), [&](auto warps, auto an_sm) {
+        return launch_skinny<MT, O, decltype(warps)::value, decltype(an_sm)::value>(a, s);
+    });
 }
 
 // More tokens than the weight-streaming kernel takes at once: 256 x 256 tiles on pairs of SMs, or narrower tiles with K cut over a cluster,

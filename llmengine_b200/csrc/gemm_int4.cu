@@ -238,10 +238,9 @@ int launch_skinny(const Args& a, cudaStream_t s) {
 }
 template <int MT, int RUNS, bool ZEROS>
 int launch_skinny(const Args& a, cudaStream_t s) {
-    const stream::Shares by = stream::sharing((a.N + 15) / 16, (a.K + 2 * BLOCK_K - 1) / (2 * BLOCK_K), sm_count());
-    if (by.warps == 16) return launch_skinny<MT, RUNS, ZEROS, 16, 16>(a, s);
-    if (by.warps == 8) return by.an_sm == 16 ? launch_skinny<MT, RUNS, ZEROS, 8, 16>(a, s) : launch_skinny<MT, RUNS, ZEROS, 8, 24>(a, s);
-    return by.warps == 4 ? launch_skinny<MT, RUNS, ZEROS, 4, 24>(a, s) : launch_skinny<MT, RUNS, ZEROS, 2, 24>(a, s);
+    return stream::with(stream::sharing((a.N + 15) / 16, (a.K + 2 * BLOCK_K - 1) / (2 * BLOCK_K), sm_count()), [&](auto warps, auto an_sm) {
+        return launch_skinny<MT, RUNS, ZEROS, decltype(warps)::value, decltype(an_sm)::value>(a, s);
+    });
 }
 
 // More tokens than the weight-streaming kernel takes at once: pairs of SMs, or single ones with K cut over a cluster, whichever a model of its

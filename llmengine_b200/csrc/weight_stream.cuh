@@ -3,8 +3,8 @@
 // A warp owns 16 weight rows and walks over them in pieces of 128 bytes a row; lane (r, quad) = (lane / 4, lane % 4) needs of every piece the
 // 16 bytes at quad * 16 and at 64 + quad * 16 of rows r and r + 8.  The pieces of the next steps lie in a ring in shared memory, brought by
 // asynchronous copies: every lane copies what it will read itself, so nothing has to be shared and no barrier is met, and how much is under
-// way does not cost registers.  (With the pieces in registers a warp's loads and its arithmetic took turns: 24576 x 4096 in 4 bits, one
-// token, 18.1 us, where the loads alone take 10.1.)
+// way does not cost registers.  (24576 x 4096 in 4 bits, one token: 13.9 us, the loads alone 10.1; with the pieces in registers a warp's loads and
+// its arithmetic took turns, 18.1 us.  A ring of three, four or six steps gains nothing.)
 // Where the row groups alone do not fill the GPU, several warps share a group: warp p of n takes the pieces p, p + n, ..., and their sums are
 // added in the order of the warps.  How many share follows from the weights' shape alone, so a token's result does not depend on the others.
 // A block is one group: blocks of several came out less even over the SMs.
@@ -40,17 +40,38 @@ struct Ring {
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// How many warps share a row group, and how many warps an SM should hold.  Few groups: many warps each; and where two blocks an SM hold all
-// groups, no SM should take three (256 groups of 12,288 4-bit values, one token: 9.4 us with room for two blocks of eight warps, 10.8 with room
-// for three; 384 groups of 4,096: 6.0 with two, 5.3 with three).  Many groups: few warps each, so that the last blocks to run are short
-// (1,536 groups of 4,096: 14.1 us with two warps, 15.3 with four, 15.4 with eight).
+// How many warps share a row group, and how many warps an SM should hold.  Few groups: many warps each; many groups: few warps each, so that the
+// last blocks to run are short (1,536 groups of 4,096 4-bit values, one token: 14.1 us with two warps, 15.3 with four, 15.4 with eight).  Of the
+// warps an SM may hold those that leave the last round of blocks fullest, and the fewest of these: the others' room is registers (4-bit values in
+// groups of 32 with zero points, eight tokens: 448 groups of 5,120 9.8 us with room for four blocks of four warps, 12.6 for five, 14.9 for six; 864
+// groups of 5,120 17.9, 23.7 and 16.5; 2,000 groups of 4,096, two warps each, 27.3 us with room for eight blocks, 37.6 for ten, 44.7 for twelve.  256
+// groups of 12,288, groups of 128, one token: 9.4 us with room for two blocks of eight warps, 10.8 for three).
 struct Shares { int warps, an_sm; };
 inline Shares sharing(int groups, int pieces, int sms) {
-    if (groups <= sms && pieces >= 16) return {16, 16};
-    if (groups <= 2 * sms) return {8, 16};
-    if (groups <= 3 * sms) return {8, 24};
-    if (groups <= 6 * sms) return {4, 24};
-    return {2, 24};
+    const int each = (groups + sms - 1) / sms;              // blocks that an SM should hold
+    if (each <= 1 && pieces >= 16) return {16, 16};
+    if (each <= 3) return {8, each <= 2 ? 16 : 24};
+    Shares by{each <= 6 ? 4 : 2, 0};
+    double fullest = 0.0;
+    for (int an_sm = 16; an_sm <= 24; an_sm += 4) {
+        const long long held = (long long)an_sm / by.warps * sms, rounds = (groups + held - 1) / held;
+        const double full = (double)groups / (double)(rounds * held);
+        if (full > fullest) { fullest = full; by.an_sm = an_sm; }
+    }
+    return by;
+}
+// launch(warps, an_sm), both as compile-time numbers
+template <typename F>
+int with(Shares by, F launch) {
+    using std::integral_constant;
+    auto held = [&](auto warps) {
+        if (by.an_sm == 16) return launch(warps, integral_constant<int, 16>{});
+        if (by.an_sm == 20) return launch(warps, integral_constant<int, 20>{});
+        return launch(warps, integral_constant<int, 24>{});
+    };
+    if (by.warps == 16) return launch(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+    if (by.warps == 8) return by.an_sm == 16 ? launch(integral_constant<int, 8>{}, integral_constant<int, 16>{}) : launch(integral_constant<int, 8>{}, integral_constant<int, 24>{});
+    return by.warps == 4 ? held(integral_constant<int, 4>{}) : held(integral_constant<int, 2>{});
 }
 
 }  // namespace stream
