@@ -4,8 +4,9 @@
 // Up to 16 tokens: bound by reading W once.  16 rows of W are the M side of a mma.sync.m16n8k32 tile and the tokens its N side.  The
 // order in which the k values of a dot product are added is free: within every 64 values the four lanes of a quad take 16 consecutive ones
 // each, for W and x alike, so that a lane's operands for two steps are 16 bytes of a row of W (two rows a lane), on their way through a ring
-// in shared memory (weight_stream.cuh), and one 16-byte load of a row of x.
-// More: tcgen05, the weights on the lanes of tensor memory (gemm_wide.cuh) or 256 x 256 tiles on pairs of SMs (gemm_e4m3_pair.cuh).
+// in shared memory (weight_stream.cuh), and one 16-byte load of a row of x.  8 x 6144 x 4096 6.8 us (3.7 TB/s), 8 x 24576 x 4096 19.5 (5.2 TB/s).
+// More: tcgen05, the weights on the lanes of tensor memory (gemm_wide.cuh: 77 x 4096 x 12288 14.6 us, 3.6 TB/s) or 256 x 256 tiles on pairs of
+// SMs (gemm_e4m3_pair.cuh: 2048 x 24576 x 4096 144 us, 2.86 PFLOP/s).
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
 #include <cuda.h>

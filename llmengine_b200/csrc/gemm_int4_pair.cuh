@@ -12,6 +12,7 @@
 //     cycles from step to step, a third of them waits and messages: two sets were slower than the instructions, which take 768 at 192 tokens);
 //   * four warps read the block's half of the accumulator, which is double-buffered, and store it, a token's 32 neighbouring values at a time
 //     (1999 x 8192 x 256, little else: 17 us; through shared memory and TMA 25).
+// 1900 x 7168 x 5120 takes 92 us (1.51 PFLOP/s), the tensor pipe busy for 88 % of the time.
 // The accumulators take 2 NT columns of tensor memory and the weights the rest, 64 columns a step: NT is at most 192.
 // All waits are bounded (umma.cuh).
 #pragma once

@@ -9,6 +9,8 @@
 //   * one warp issues the instructions (128 x NT x 16 bfloat16, 128 x NT x 32 e4m3) into one accumulator in tensor memory;
 //   * at the end eight warps read the accumulator.  One segment: they store it.  Several: each block leaves its sums in shared memory and
 //     adds a share of the outputs over the cluster's blocks in their order.
+// Bound by the weights' way from memory where the tokens are few, by what a block brings from L2 and, with 4 bits, by the making of numbers where
+// they are more: 77 x 4096 x 12288 in 8 bits 14.6 us (3.6 TB/s), 40 / 200 x 7168 x 5120 in 8 bits 11.3 / 15.4 us, in 4 bits 14.1 / 22.3.
 // All waits are bounded (umma.cuh).
 #pragma once
 
