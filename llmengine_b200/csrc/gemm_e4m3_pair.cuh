@@ -191,15 +191,20 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                             if (m0 < a.M && col < a.N) tma_store_2d(&map_o, buf, col, m0);
                             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
-                    } else {
-                        // an output whose rows begin anywhere: value by value, the lanes along a row
+                    } else if (h == PIECES - 1) {
+                        // an output whose rows begin anywhere: value by value, the 32 lanes along a row (all rows wherever there are so many)
                         __syncwarp();
-                        const int at = lane % COLS, last = min(32, a.M - m0);
-                        O* to = reinterpret_cast<O*>(a.out) + (long long)(m0 + lane / COLS) * a.ldo + col + at;
-                        if (col + at < a.N)
-#pragma unroll 8
-                            for (int r = lane / COLS; r < last; r += PIECES, to += PIECES * a.ldo)
-                                *to = *reinterpret_cast<const O*>(buf + r * 64 + ((((at * (int)sizeof(O)) >> 4) ^ ((r >> 1) & 3)) << 4) + ((at * (int)sizeof(O)) & 15));
+                        const int last = a.M - m0, left = a.N - (n0 + j * 32), chunk = lane * (int)sizeof(O) % 64 / 16, byte = lane * (int)sizeof(O) % 16;
+                        const unsigned char* from = (PIECES == 2 ? own + lane / 16 * 2048 : buf) + byte;
+                        O* to = reinterpret_cast<O*>(a.out) + (long long)m0 * a.ldo + (n0 + j * 32 + lane);
+                        if (lane < left) {
+                            if (last >= 32) {
+#pragma unroll
+                                for (int r = 0; r < 32; ++r, to += a.ldo) *to = *reinterpret_cast<const O*>(from + r * 64 + ((chunk ^ (r >> 1 & 3)) << 4));
+                            } else {
+                                for (int r = 0; r < last; ++r, to += a.ldo) *to = *reinterpret_cast<const O*>(from + r * 64 + ((chunk ^ (r >> 1 & 3)) << 4));
+                            }
+                        }
                         __syncwarp();
                     }
                 }
