@@ -389,7 +389,8 @@ int clusters_held(int segments, int per_sm) {
 // codes keeps an SM busy for 850.  Starting and ending a block cost about 4,000 cycles and 22 for every token, the cluster's sums 3,000 and 10.
 // Over 42 products of 40 to 1,600 tokens and all of their tilings the model is off by 12 % (standard deviation), and its choice took 1 % longer than
 // the best with 8 bits, 2 % with 4.  (200 x 4096 x 4096 in 8 bits, tiles of 208 tokens in four segments, 10.7 us; 96 x 7168 x 5120 in 4 bits, two
-// segments, 15.6, where tiles of 48, two blocks an SM, take 31.)
+// segments, 15.6, where tiles of 48, two blocks an SM, take 31.  Tiles a quarter as wide as the widest are for few weight rows: 2048 x 264 x 1616 in
+// 8 bits 7.0 us, with tiles of 192 to 256 alone 9.1.)
 template <bool INT4, int RUNS, bool ZEROS>
 int shape(Args& g, double* cycles) {
     const int steps = (g.K + STEP - 1) / STEP, n_tiles = (g.N + BM - 1) / BM, w_bytes = INT4 ? BM * STEP / 2 : BM * STEP, x_width = STEP * (INT4 ? 2 : 1);
@@ -397,11 +398,11 @@ int shape(Args& g, double* cycles) {
     static LlmeGrants grants;
     if (cudaError_t e = llme_grant_smem(grants, wide_kernel<INT4, RUNS, ZEROS>, MOST_SMEM)) LLME_REFUSE("gemm_wide: cannot reserve %zu bytes of shared memory: %s", MOST_SMEM, cudaGetErrorString(e));
     double best = -1.0;
-    for (int m_tiles = least; m_tiles <= least + 3; ++m_tiles) {
+    for (int m_tiles = least; m_tiles <= 4 * least + 3; m_tiles += m_tiles < least + 3 ? 1 : (least + 3) / 2) {
         const int nt = ((g.M + m_tiles - 1) / m_tiles + 15) / 16 * 16;
         const long long tiles = (long long)n_tiles * ((g.M + nt - 1) / nt);
         for (int per_sm = 1; per_sm <= (nt <= 64 ? 2 : 1); ++per_sm)
-            for (int segments = 1; segments <= MOST_SEGMENTS && segments <= steps; ++segments) {
+            for (int segments = 1; segments <= MOST_SEGMENTS && segments <= steps && (segments == 1 || tiles < sm_count()); ++segments) {
                 const int each = (steps + segments - 1) / segments;
                 if ((steps + each - 1) / each != segments) continue;
                 const int held = clusters_held<INT4, RUNS, ZEROS>(segments, per_sm);
