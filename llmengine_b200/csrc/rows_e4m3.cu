@@ -172,6 +172,11 @@ __device__ __forceinline__ float row_scale(float top, float r) {
     return (m >= LEAST ? m : (m < LEAST ? LEAST : m)) / LARGEST;       // (NaN stays)
 }
 
+// Whether the factor r / a that takes a norm's values to e4m3 is above the largest 32-bit number: in rows near zero under an eps below 2.8e-12, where
+// r is above 6.0e5 and a may be as small as 2^-100 / 448.  The values then take the two parts one after the other: r makes of them the root of the
+// row's width at most, and 1 / a is at most 448 2^100.  (Both parts for every row: 1,999 x 5,120 18.9 us, with this question 18.6.)
+__device__ __forceinline__ bool in_two_parts(float f) { return f > 3.402823466e38f; }
+
 // Sum and largest over the threads of a row: the lanes of a warp, or a block's.
 template <bool BLOCK>
 __device__ __forceinline__ void meet(float& ss, float& top, float* sums, unsigned* tops) {
@@ -219,8 +224,16 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 640) : 128) quantise_
             }
         }
         meet<BLOCK>(ss, top, sums, tops);
-        const float r = 1.0f / sqrtf(ss / (float)size + src.eps), a = row_scale(top, r), f = r / a;
+        const float r = 1.0f / sqrtf(ss / (float)size + src.eps), a = row_scale(top, r);
+        float f = r / a;
         if (t == 0) scales[row] = a;
+        if (in_two_parts(f)) {
+            f = 1.0f / a;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[k][i] *= r;
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int j = (t + k * step) * N;
@@ -278,14 +291,16 @@ __global__ void __launch_bounds__(512) quantise_long_kernel(const Src src, unsig
     meet<true>(ss, top, sums, tops);
     float r = 1.0f;
     if constexpr (Src::NORM) r = 1.0f / sqrtf(ss / (float)size + src.eps);
-    const float a = row_scale(top, r), f = r / a;
+    const float a = row_scale(top, r);
+    float f = r / a, first = 1.0f;
+    if (Src::NORM && in_two_parts(f)) { f = 1.0f / a; first = r; }
     if (threadIdx.x == 0) scales[row] = a;
     for (int j = N * (int)threadIdx.x; j < size; j += N * (int)blockDim.x) {
         if constexpr (Src::NORM) {
             Piece<float, N> t;
             t.load((src.delta ? src.total : src.x) + (long long)row * size + j);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = (t.at(i) * f) * to_f32(src.gain[j + i]);
+            for (int i = 0; i < N; ++i) v[i] = (t.at(i) * first * f) * to_f32(src.gain[j + i]);
         } else {
             typename Src::template Raw<N> raw;
             src.template fetch<N>(row, j, raw);
