@@ -101,14 +101,15 @@ template <typename T> struct FromRows {
         for (int i = 0; i < N; ++i) v[i] = r.at(i);
     }
 };
-// 1 / (1 + exp(-g)) for a g that has been through bfloat16, from the hardware's exponential and reciprocal: 2^-22 and 2^-23 of the value (and the
-// rounding of the exponent), far below the 2^-4 of what it goes into.  Arithmetic bounds the gate's kernel: with the corrected reciprocal and
-// the exponential for subnormal results 2,048 x 17,408 took 39.0 us.
-__device__ __forceinline__ float sigmoid_fast(float g) {
+// silu(g) for a g that has been through bfloat16, from the hardware's exponential and reciprocal: 2^-22 and 2^-23 of the value (and the rounding of
+// the exponent), far below the 2^-4 of what it goes into.  As (g / 4) / (1 / 4 + exp(-g) / 4): the reciprocal of 1 + exp(-g) is below 2^-126 for g
+// under -87.3, and would count as zero, a quarter's is a number wherever exp(-g) is one in 32 bits (below -88.7 it is not, and silu is 0).  Arithmetic
+// bounds the gate's kernel: with the corrected reciprocal and the exponential for subnormal results 2,048 x 17,408 took 39.0 us.
+__device__ __forceinline__ float silu_fast(float g) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -1.4426950408889634f, -2.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.25f + e));
+    return (0.25f * g) * r;
 }
 template <typename T> struct FromGate {
     static constexpr bool NORM = false, EXACT = false;
@@ -123,7 +124,7 @@ template <typename T> struct FromGate {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float g = r.gate.at(i);
-            v[i] = (sizeof(T) == 2 ? g * sigmoid_fast(g) : g / (1.0f + expf(-g))) * r.up.at(i);
+            v[i] = (sizeof(T) == 2 ? silu_fast(g) : g / (1.0f + expf(-g))) * r.up.at(i);
         }
     }
 };
