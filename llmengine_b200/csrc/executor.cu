@@ -455,9 +455,10 @@ int op_linear_e4m3(LlmeExecutor& ex, const LlmeLinearE4m3Op& o, const LlmeStep& 
 }
 
 int op_linear_int4(LlmeExecutor& ex, const LlmeLinearInt4Op& o, const LlmeStep& s, cudaStream_t st) {
-    auto* f = (GemmInt4Fn)ex.find("gemm_int4");
+    const char* name = o.out_dtype == LLME_DT_F32 ? "gemm_int4_f32" : "gemm_int4";
+    auto* f = (GemmInt4Fn)ex.find(name);
     if (!f) return ex.fail("no product with 4-bit weights is registered");
-    return ex.launched(f(o.x, o.ldx, o.w, o.ldw, o.scales, o.zeros, o.lds, o.group, o.out, o.ldo, s.num_tokens, o.n, o.k, st), "gemm_int4");
+    return ex.launched(f(o.x, o.ldx, o.w, o.ldw, o.scales, o.zeros, o.lds, o.group, o.out, o.ldo, s.num_tokens, o.n, o.k, st), name);
 }
 
 int op_swiglu(LlmeExecutor& ex, const LlmeSwigluOp& o, const LlmeStep& s, cudaStream_t st) {

@@ -38,7 +38,7 @@ struct Args {
     const bf16* x; long long ldx;
     const unsigned char* w; long long ldw;                  // bytes from row to row
     const bf16* scales; const unsigned char* zeros; long long lds;      // values from row to row of both
-    bf16* out; long long ldo;
+    void* out; int out_f32; long long ldo;                  // 32-bit or bfloat16
     int M, N, K;
     int together;                                           // scales and zero points that lie on their size: 2 a piece's, 1 a block's, 0 one
 };
@@ -222,7 +222,8 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
         float v = red[tok][i & 15];
 #pragma unroll
         for (int w = 1; w < SHARE; ++w) v += red[w * MT * 8 + tok][i & 15];
-        a.out[(size_t)tok * a.ldo + row] = __float2bfloat16_rn(v);
+        if (a.out_f32) reinterpret_cast<float*>(a.out)[(size_t)tok * a.ldo + row] = v;
+        else reinterpret_cast<bf16*>(a.out)[(size_t)tok * a.ldo + row] = __float2bfloat16_rn(v);
     }
 }
 
@@ -251,17 +252,17 @@ int launch_wide(const Args& a, cudaStream_t s) {
     alignas(64) CUtensorMap mw, mx;
     if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
     wide::Args g{};
-    g.out = a.out; g.ldo = a.ldo;
+    g.out = a.out; g.ldo = a.ldo; g.out_f32 = a.out_f32;
     g.M = a.M; g.N = a.N; g.K = a.K;
     g.scales = a.scales; g.zeros = a.zeros; g.lds = a.lds;
-    g.vec_out = (uintptr_t)a.out % 8 == 0 && a.ldo % 4 == 0;
+    g.vec_out = (uintptr_t)a.out % (a.out_f32 ? 16 : 8) == 0 && a.ldo % 4 == 0;
     double single, paired;
     if (int rc = wide::shape<true, RUNS, ZEROS>(g, &single)) return rc;
     pair::PairArgs p{a.out, a.ldo, a.M, a.N, a.K, 0, 0, 0, a.scales, a.zeros, a.lds};
     if (int rc = pair::shape<RUNS, ZEROS>(p, &paired)) return rc;
     if (g_form == 2 || (g_form == 0 && paired < single)) {
         if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, p.nt / 2, 64)) return rc;
-        return pair::launch<RUNS, ZEROS>(mw, mx, p, s);
+        return a.out_f32 ? pair::launch<RUNS, ZEROS, float>(mw, mx, p, s) : pair::launch<RUNS, ZEROS, bf16>(mw, mx, p, s);
     }
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, g.nt, 64)) return rc;
     return wide::launch<true, RUNS, ZEROS>(mw, mx, g, s);
@@ -275,13 +276,9 @@ int launch(const Args& a, cudaStream_t s) {
 template <int RUNS>
 int launch(const Args& a, cudaStream_t s) { return a.zeros ? launch<RUNS, true>(a, s) : launch<RUNS, false>(a, s); }
 
-}  // namespace
-
-// x [M,K] bfloat16 with row stride ldx (elements, a multiple of 8; K too); w the codes [N, ceil(K / 128) * 64] with row stride ldw (bytes,
-// a multiple of 16); scales [N, ceil(K / group)] bfloat16 and zeros of the same shape (values 0..15) or NULL, row stride lds; out [M,N]
-// bfloat16, row stride ldo.
-LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds,
-                            int group, void* out, long long ldo, int M, int N, int K, cudaStream_t stream) {
+// What both entry points check and launch.
+int product(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds, int group, void* out, int out_f32, long long ldo,
+            int M, int N, int K, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !w || !scales || !out) LLME_REFUSE("gemm_int4: null pointer");
     if (K <= 0 || K % 8 || ldx % 8 || ldx < K) LLME_REFUSE("gemm_int4: K=%d ldx=%lld is not supported (multiples of 8, rows that do not overlap)", K, ldx);
@@ -291,14 +288,29 @@ LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long lo
     if (((uintptr_t)x | (uintptr_t)w) % 16) LLME_REFUSE("gemm_int4: operands must be 16-byte aligned");
     if (ldo < N) LLME_REFUSE("gemm_int4: output row stride shorter than the row");
     const long long groups = (K + group - 1LL) / group;
-    if (meets(span(out, M, N, ldo, 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
+    if (meets(span(out, M, N, ldo, out_f32 ? 4 : 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
         LLME_REFUSE("gemm_int4: the output lies over an operand");
-    Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, (bf16*)out, ldo, M, N, K, 0};
+    Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, out, out_f32, ldo, M, N, K, 0};
     auto aligned = [&](int count) { return lds % count == 0 && (uintptr_t)scales % (2 * count) == 0 && (uintptr_t)zeros % count == 0; };
     a.together = aligned(256 / group) ? 2 : (aligned(128 / group) ? 1 : 0);
     if (group == 32) return launch<1>(a, stream);
     if (group == 64) return launch<2>(a, stream);
     return launch<4>(a, stream);
+}
+
+}  // namespace
+
+// x [M,K] bfloat16 with row stride ldx (elements, a multiple of 8; K too); w the codes [N, ceil(K / 128) * 64] with row stride ldw (bytes,
+// a multiple of 16); scales [N, ceil(K / group)] bfloat16 and zeros of the same shape (values 0..15) or NULL, row stride lds; out [M,N]
+// bfloat16, row stride ldo.
+LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds,
+                            int group, void* out, long long ldo, int M, int N, int K, cudaStream_t stream) {
+    return product(x, ldx, w, ldw, scales, zeros, lds, group, out, 0, ldo, M, N, K, stream);
+}
+// The same with a 32-bit out: a sum on its way into the residual stream.
+LLME_API int llme_gemm_int4_f32(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds,
+                                int group, void* out, long long ldo, int M, int N, int K, cudaStream_t stream) {
+    return product(x, ldx, w, ldw, scales, zeros, lds, group, out, 1, ldo, M, N, K, stream);
 }
 
 // More than 16 tokens: 0 (the default): whichever kernel should be faster; 1: single SMs, K cut over clusters; 2: pairs of SMs.  For tests and

@@ -25,7 +25,7 @@ constexpr int BLOCK = (FIRST_OUT + OUT_WARPS) * 32, W_BYTES = BM * STEP / 2, TIL
 constexpr unsigned TMEM = 512;
 
 struct PairArgs {
-    bf16* out; long long ldo;
+    void* out; long long ldo;
     int M, N, K, nt, stages, w_stages;
     const bf16* scales; const unsigned char* zeros; long long lds;
 };
@@ -55,7 +55,8 @@ __device__ __forceinline__ void mma_step(unsigned d, unsigned w, unsigned long l
         ::"r"(d), "r"(w), "l"(x0), "l"(x1), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-template <int RUNS, bool ZEROS>
+// O: the output's type, float or bfloat16
+template <int RUNS, bool ZEROS, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(BLOCK, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PairArgs g) {
     extern __shared__ unsigned char smem_raw[];
@@ -227,14 +228,14 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             auto put = [&](const unsigned (&v)[32], int j) {
                 if (n >= g.N) return;
                 const int left = g.M - m0 - j;
-                bf16* to = g.out + (long long)(m0 + j) * g.ldo + n;
+                O* to = reinterpret_cast<O*>(g.out) + (long long)(m0 + j) * g.ldo + n;
                 if (left >= 32) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e, to += g.ldo) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+                    for (int e = 0; e < 32; ++e, to += g.ldo) *to = from_f32<O>(__uint_as_float(v[e]));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e, to += g.ldo)
-                        if (e < left) *to = __float2bfloat16_rn(__uint_as_float(v[e]));
+                        if (e < left) *to = from_f32<O>(__uint_as_float(v[e]));
                 }
             };
             // the next values are on their way out of tensor memory while these are stored; behind the last the accumulator may be filled again
@@ -273,7 +274,14 @@ pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
 
 inline size_t smem_of(int nt, int stages) { return 1024 + (size_t)stages * (W_BYTES + (size_t)nt / 2 * STEP * 2) + sizeof(Barriers); }
 
-// How many pairs the GPU holds at once: the two blocks of a pair need two free SMs of one GPC.
+template <int RUNS, bool ZEROS, typename O>
+int grant() {
+    static LlmeGrants grants;
+    if (cudaError_t e = llme_grant_smem(grants, pair_kernel<RUNS, ZEROS, O>, wide::MOST_SMEM)) LLME_REFUSE("gemm_int4: cannot reserve %zu bytes of shared memory: %s", wide::MOST_SMEM, cudaGetErrorString(e));
+    return 0;
+}
+
+// How many pairs the GPU holds at once, of whichever output type (asked of bfloat16's kernel): the two blocks of a pair need two free SMs of one GPC.
 template <int RUNS, bool ZEROS>
 int pairs_held() {
     static std::atomic<int> known{0};
@@ -283,7 +291,7 @@ int pairs_held() {
     cfg.gridDim = dim3(2 * 1024, 1, 1);
     cfg.blockDim = dim3(BLOCK);
     cfg.dynamicSmemBytes = wide::MOST_SMEM;
-    if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<RUNS, ZEROS>, &cfg) != cudaSuccess || n <= 0 || n > sm_count() / 2) {
+    if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<RUNS, ZEROS, bf16>, &cfg) != cudaSuccess || n <= 0 || n > sm_count() / 2) {
         cudaGetLastError();
         n = sm_count() / 2;
     }
@@ -297,8 +305,7 @@ int pairs_held() {
 // every token.
 template <int RUNS, bool ZEROS>
 int shape(PairArgs& g, double* cycles) {
-    static LlmeGrants grants;
-    if (cudaError_t e = llme_grant_smem(grants, pair_kernel<RUNS, ZEROS>, wide::MOST_SMEM)) LLME_REFUSE("gemm_int4: cannot reserve %zu bytes of shared memory: %s", wide::MOST_SMEM, cudaGetErrorString(e));
+    if (int rc = grant<RUNS, ZEROS, bf16>()) return rc;
     const int held = pairs_held<RUNS, ZEROS>(), n_tiles = (g.N + TILE_N - 1) / TILE_N;
     *cycles = -1.0;
     for (int nt = 64; nt <= MOST_NT; nt += 32) {
@@ -314,11 +321,12 @@ int shape(PairArgs& g, double* cycles) {
     return 0;
 }
 
-template <int RUNS, bool ZEROS>
+template <int RUNS, bool ZEROS, typename O>
 int launch(const CUtensorMap& mw, const CUtensorMap& mx, const PairArgs& g, cudaStream_t s) {
+    if (int rc = grant<RUNS, ZEROS, O>()) return rc;
     const long long tiles = (long long)((g.M + g.nt - 1) / g.nt) * ((g.N + TILE_N - 1) / TILE_N);
     const int held = pairs_held<RUNS, ZEROS>();
-    llme_launch(pair_kernel<RUNS, ZEROS>, dim3((unsigned)(tiles < held ? tiles : held) * 2), dim3(BLOCK), smem_of(g.nt, g.stages), s, mw, mx, g);
+    llme_launch(pair_kernel<RUNS, ZEROS, O>, dim3((unsigned)(tiles < held ? tiles : held) * 2), dim3(BLOCK), smem_of(g.nt, g.stages), s, mw, mx, g);
     LLME_LAUNCH_STATUS();
 }
 

@@ -268,7 +268,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = f[e] * __shfl_sync(0xffffffffu, scales, (j & 31) + e) * ws;
             }
-            if (!INT4 && g.out_f32) {
+            if (g.out_f32) {
                 store8(reinterpret_cast<float*>(g.out) + (long long)(first + j) * g.ldo + n, g.ldo, left - j, f);
             } else {
                 store8(reinterpret_cast<bf16*>(g.out) + (long long)(first + j) * g.ldo + n, g.ldo, left - j, f);

@@ -126,7 +126,7 @@ class Plan:
     def linear_int4(self, x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int,
                     out: torch.Tensor) -> None:
         """out = x w^T for the step's tokens with weights of 4 bits: w[n, k] = scales[n, k // group] (code[n, k] - zeros[n, k // group]),
-        codes as weights.quantize.pack_int4 lays them; `zeros` None: 8 everywhere."""
+        codes as weights.quantize.pack_int4 lays them; `zeros` None: 8 everywhere.  x bfloat16, out 32-bit or bfloat16."""
         self._add("linear_int4", x=x, w=w, scales=scales, zeros=zeros, group=int(group), out=out)
 
     def swiglu(self, gate_up: torch.Tensor, out: torch.Tensor) -> None:

@@ -170,13 +170,13 @@ typedef struct LlmeLinearE4m3Op {
     int n, k;
 } LlmeLinearE4m3Op;
 
-/* out = x w^T for bfloat16 x and out and 4-bit weights, w[j, i] = scales[j, i / group] (code - zeros[j, i / group]) (csrc/gemm_int4.cu);
+/* out = x w^T for bfloat16 x, 32-bit or bfloat16 out and 4-bit weights, w[j, i] = scales[j, i / group] (code - zeros[j, i / group]) (csrc/gemm_int4.cu);
  * zeros NULL: 8 everywhere. */
 typedef struct LlmeLinearInt4Op {
     const void* x; long long ldx;
     const void* w; long long ldw;                        /* codes: bytes from row to row */
     const void* scales; const void* zeros; long long lds; /* bfloat16, bytes */
-    void* out; long long ldo;
+    void* out; long long ldo; int out_dtype;
     int group, n, k;
 } LlmeLinearInt4Op;
 

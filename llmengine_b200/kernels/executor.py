@@ -83,7 +83,7 @@ class LinearE4m3Op(Structure):
 
 class LinearInt4Op(Structure):
     _fields_ = [("x", c_void_p), ("ldx", c_longlong), ("w", c_void_p), ("ldw", c_longlong), ("scales", c_void_p), ("zeros", c_void_p),
-                ("lds", c_longlong), ("out", c_void_p), ("ldo", c_longlong), ("group", c_int), ("n", c_int), ("k", c_int)]
+                ("lds", c_longlong), ("out", c_void_p), ("ldo", c_longlong), ("out_dtype", c_int), ("group", c_int), ("n", c_int), ("k", c_int)]
 
 
 class SwigluOp(Structure):
@@ -385,13 +385,13 @@ def records(op, keep: List[Any]):
                                             out.stride(0), code(out.dtype), w.shape[0], w.shape[1])
     if k == "linear_int4":
         x, w, sc, z, out = a["x"], a["w"], a["scales"], a["zeros"], a["out"]
-        assert x.dtype == out.dtype == torch.bfloat16 and x.stride(1) == 1 and out.stride(1) == 1 and out.shape[1] == w.shape[0]
+        assert x.dtype == torch.bfloat16 and x.stride(1) == 1 and out.stride(1) == 1 and out.shape[1] == w.shape[0]
         assert w.dtype == torch.uint8 and w.stride(1) == 1 and w.shape[1] == -(-x.shape[1] // 128) * 64
         groups = (w.shape[0], -(-x.shape[1] // a["group"]))
         assert sc.dtype == torch.bfloat16 and sc.is_contiguous() and sc.shape == groups
         assert z is None or (z.dtype == torch.uint8 and z.is_contiguous() and z.shape == groups)
         return OP_LINEAR_INT4, LinearInt4Op(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), sc.data_ptr(), ptr(z), groups[1],
-                                            out.data_ptr(), out.stride(0), a["group"], w.shape[0], x.shape[1])
+                                            out.data_ptr(), out.stride(0), code(out.dtype), a["group"], w.shape[0], x.shape[1])
     if k == "swiglu":
         gu, out = a["gate_up"], a["out"]
         assert gu.is_contiguous() and out.is_contiguous() and gu.dtype == out.dtype and gu.shape[1] == 2 * out.shape[1]

@@ -227,7 +227,7 @@ class CudaOps:
                          "gemm_tc_act": "llme_gemm_tc_act_bf16", "gemm_tc_gated": "llme_gemm_tc_gated_bf16"},
         "rows_e4m3": {"rmsnorm_e4m3": "llme_rmsnorm_e4m3", "rows_e4m3": "llme_rows_e4m3", "swiglu_e4m3": "llme_swiglu_e4m3"},
         "gemm_e4m3": {"gemm_e4m3": "llme_gemm_e4m3"},
-        "gemm_int4": {"gemm_int4": "llme_gemm_int4"},
+        "gemm_int4": {"gemm_int4": "llme_gemm_int4", "gemm_int4_f32": "llme_gemm_int4_f32"},
         "attention_plain": {"attention_plain": "llme_attention_plain"},
         "attention_fast": {"attention_portion/{hd}": "llme_attention_portion", "attention_decode/{hd}": "llme_attention_decode",
                            "attention_decode_fused/{hd}": "llme_attention_decode_fused",
@@ -714,7 +714,7 @@ class CudaOps:
         """out[m, n] = sum over k of x[m, k] scales[n, g] (c[n, k] - zeros[n, g]), g = k // group: x [M, K] and out [M, N] bfloat16; `w`
         uint8 [N, ceil(K / 128) * 64], the codes c as weights.quantize.pack_int4 lays them; scales [N, ceil(K / group)] bfloat16 for a
         group of 32, 64 or 128; zeros uint8 of that shape with values 0..15 (None: 8 everywhere).  Sums are 32-bit.  K is a multiple
-        of 8, the rows of x and w begin on 16 bytes (any such row stride)."""
+        of 8, the rows of x and w begin on 16 bytes (any such row stride).  (Into 32 bits: the plan's record, `Plan.linear_int4`.)"""
         what, d = "linear_int4", self._device_index
         M, K = self._operand(what, "x", x, _BF16S).shape
         if not (w.get_device() == d == scales.get_device() and out.get_device() == d and w.dtype is _BYTE and scales.dtype is _BF16T

@@ -11,7 +11,7 @@ from ..config.spec import PartSpec
 from ..engine.plan import Plan
 from dataclasses import dataclass
 
-from .low_bit import emit_linear, hold, result_dtype
+from .low_bit import emit_linear, hold
 from .base import (PagedAndStateSpec, PagedAndStateView, PagedKVSpec, Part, Runtime, StatesSpec, WeightSpec, build_part,
                    register_part, run_alone)
 
@@ -102,7 +102,7 @@ class GQAttention(Part):
             if writes:
                 plan.qkv_post(q_in=None, k_in=k, v_in=qkv[:, qs + kvs:], **common)
             plan.attend(q=q, out=out, window=self.window, scale=self.scale, scratch=scratch, **common)
-        delta = rt.workspace("mixer_out", self.hidden, result_dtype(rt))
+        delta = rt.workspace("mixer_out", self.hidden, torch.float32)
         emit_linear(plan, rt, out, self.w_o, delta, "attn_rows8")
         return delta
 

@@ -7,7 +7,7 @@ import torch
 
 from ..engine.plan import Plan
 from .base import Part, Runtime, WeightSpec, register_part, run_alone
-from .low_bit import emit_linear, hold, result_dtype, rows8_place
+from .low_bit import emit_linear, hold, rows8_place
 
 
 @register_part("feed_forward", "swiglu")
@@ -38,7 +38,7 @@ class SwiGLU(Part):
     def emit(self, plan: Plan, h: torch.Tensor) -> torch.Tensor:
         rt = self.rt
         gate_up = rt.workspace("gate_up", 2 * self.inter, rt.dtype)
-        delta = rt.workspace("ffn_out", self.hidden, result_dtype(rt))
+        delta = rt.workspace("ffn_out", self.hidden, torch.float32)
         if rt.weights == "e4m3":
             emit_linear(plan, rt, h, self.w_gate_up, gate_up, "normed_rows8")
             act = rows8_place(rt, "act_rows8", self.inter)

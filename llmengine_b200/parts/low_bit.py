@@ -65,11 +65,6 @@ def hold(rt: Runtime, w: torch.Tensor, name: str) -> Weight:
         raise ValueError(f"{name}: {e}") from None
 
 
-def result_dtype(rt: Runtime) -> torch.dtype:
-    """Type of a sublayer's result on its way into the residual stream: 32-bit; bfloat16 from 4-bit weights, whose products hold no more."""
-    return torch.bfloat16 if rt.weights == "int4" else torch.float32
-
-
 def rows8_place(rt: Runtime, name: str, size: int) -> Rows8:
     return Rows8(rt.workspace(name, size, torch.float8_e4m3fn), rt.workspace(name + "_scales", 1, torch.float32).view(-1))
 
