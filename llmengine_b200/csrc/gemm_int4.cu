@@ -38,7 +38,7 @@ struct Args {
     const bf16* x; long long ldx;
     const unsigned char* w; long long ldw;                  // bytes from row to row
     const bf16* scales; const unsigned char* zeros; long long lds;      // values from row to row of both
-    void* out; int out_f32; long long ldo;                  // 32-bit or bfloat16
+    void* out; long long ldo;
     int M, N, K;
     int together;                                           // scales and zero points that lie on their size: 2 a piece's, 1 a block's, 0 one
 };
@@ -120,8 +120,8 @@ struct Factors {
     __device__ __forceinline__ __nv_bfloat162 minus_zero(int r, int i) const { return ZEROS ? minus_zero_point(z[r][i / 4], i % 4) : __floats2bfloat162_rn(-0.125f, -0.125f); }
 };
 
-// MT: 8-token tiles.  RUNS: runs of 32 values in a group (1, 2 or 4).  SHARE: warps that share a row group; AN_SM: warps an SM is to hold.
-template <int MT, int RUNS, bool ZEROS, int SHARE, int AN_SM>
+// MT: 8-token tiles.  RUNS: runs of 32 values in a group (1, 2 or 4).  O: the output's type.  SHARE: warps that share a row group; AN_SM: warps an SM is to hold.
+template <int MT, int RUNS, bool ZEROS, typename O, int SHARE, int AN_SM>
 __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args a) {
     constexpr int GROUPS = 4 / RUNS, PAIR = 2 * BLOCK_K;          // a piece of 128 bytes is two blocks of codes
     extern __shared__ __align__(128) unsigned char rings[];
@@ -222,62 +222,62 @@ __global__ void __launch_bounds__(SHARE * 32, AN_SM / SHARE) skinny_kernel(Args 
         float v = red[tok][i & 15];
 #pragma unroll
         for (int w = 1; w < SHARE; ++w) v += red[w * MT * 8 + tok][i & 15];
-        if (a.out_f32) reinterpret_cast<float*>(a.out)[(size_t)tok * a.ldo + row] = v;
-        else reinterpret_cast<bf16*>(a.out)[(size_t)tok * a.ldo + row] = __float2bfloat16_rn(v);
+        reinterpret_cast<O*>(a.out)[(size_t)tok * a.ldo + row] = from_f32<O>(v);
     }
 }
 
-template <int MT, int RUNS, bool ZEROS, int SHARE, int AN_SM>
+template <int MT, int RUNS, bool ZEROS, typename O, int SHARE, int AN_SM>
 int launch_skinny(const Args& a, cudaStream_t s) {
     constexpr size_t smem = SHARE * stream::RING;
     static_assert(MT * 8 * 16 * 4 <= stream::RING, "the sums lie over the rings");
-    auto kernel = skinny_kernel<MT, RUNS, ZEROS, SHARE, AN_SM>;
+    auto kernel = skinny_kernel<MT, RUNS, ZEROS, O, SHARE, AN_SM>;
     static LlmeGrants grants;
     if (cudaError_t e = llme_grant_smem(grants, kernel, smem)) LLME_REFUSE("gemm_int4: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     llme_launch(kernel, dim3((a.N + 15) / 16), dim3(SHARE * 32), smem, s, a);
     LLME_LAUNCH_STATUS();
 }
-template <int MT, int RUNS, bool ZEROS>
+template <int MT, int RUNS, bool ZEROS, typename O>
 int launch_skinny(const Args& a, cudaStream_t s) {
     return stream::with(stream::sharing((a.N + 15) / 16, (a.K + 2 * BLOCK_K - 1) / (2 * BLOCK_K), sm_count()), [&](auto warps, auto an_sm) {
-        return launch_skinny<MT, RUNS, ZEROS, decltype(warps)::value, decltype(an_sm)::value>(a, s);
+        return launch_skinny<MT, RUNS, ZEROS, O, decltype(warps)::value, decltype(an_sm)::value>(a, s);
     });
 }
 
 // More tokens than the weight-streaming kernel takes at once: pairs of SMs, or single ones with K cut over a cluster, whichever a model of its
 // time says is faster.
-template <int RUNS, bool ZEROS>
+template <int RUNS, bool ZEROS, typename O>
 int launch_wide(const Args& a, cudaStream_t s) {
     const long long w_bytes = (a.K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES;
     alignas(64) CUtensorMap mw, mx;
     if (int rc = wide::make_map_swizzled(&mw, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.N, w_bytes, a.ldw, BM, BLOCK_BYTES, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
     wide::Args g{};
-    g.out = a.out; g.ldo = a.ldo; g.out_f32 = a.out_f32;
+    g.out = a.out; g.ldo = a.ldo; g.out_f32 = sizeof(O) == 4;
     g.M = a.M; g.N = a.N; g.K = a.K;
     g.scales = a.scales; g.zeros = a.zeros; g.lds = a.lds;
-    g.vec_out = (uintptr_t)a.out % (a.out_f32 ? 16 : 8) == 0 && a.ldo % 4 == 0;
+    g.vec_out = (uintptr_t)a.out % (4 * sizeof(O)) == 0 && a.ldo % 4 == 0;
     double single, paired;
     if (int rc = wide::shape<true, RUNS, ZEROS>(g, &single)) return rc;
     pair::PairArgs p{a.out, a.ldo, a.M, a.N, a.K, 0, 0, 0, a.scales, a.zeros, a.lds};
     if (int rc = pair::shape<RUNS, ZEROS>(p, &paired)) return rc;
     if (g_form == 2 || (g_form == 0 && paired < single)) {
         if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, p.nt / 2, 64)) return rc;
-        return a.out_f32 ? pair::launch<RUNS, ZEROS, float>(mw, mx, p, s) : pair::launch<RUNS, ZEROS, bf16>(mw, mx, p, s);
+        return pair::launch<RUNS, ZEROS, O>(mw, mx, p, s);
     }
     if (int rc = make_map(&mx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.M, a.K, a.ldx, g.nt, 64)) return rc;
     return wide::launch<true, RUNS, ZEROS>(mw, mx, g, s);
 }
 
-template <int RUNS, bool ZEROS>
+template <int RUNS, bool ZEROS, typename O>
 int launch(const Args& a, cudaStream_t s) {
-    if (a.M > 16) return launch_wide<RUNS, ZEROS>(a, s);
-    return a.M <= 8 ? launch_skinny<1, RUNS, ZEROS>(a, s) : launch_skinny<2, RUNS, ZEROS>(a, s);
+    if (a.M > 16) return launch_wide<RUNS, ZEROS, O>(a, s);
+    return a.M <= 8 ? launch_skinny<1, RUNS, ZEROS, O>(a, s) : launch_skinny<2, RUNS, ZEROS, O>(a, s);
 }
-template <int RUNS>
-int launch(const Args& a, cudaStream_t s) { return a.zeros ? launch<RUNS, true>(a, s) : launch<RUNS, false>(a, s); }
+template <int RUNS, typename O>
+int launch(const Args& a, cudaStream_t s) { return a.zeros ? launch<RUNS, true, O>(a, s) : launch<RUNS, false, O>(a, s); }
 
-// What both entry points check and launch.
-int product(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds, int group, void* out, int out_f32, long long ldo,
+// What both entry points check and launch; O: the output's type.
+template <typename O>
+int product(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds, int group, void* out, long long ldo,
             int M, int N, int K, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !w || !scales || !out) LLME_REFUSE("gemm_int4: null pointer");
@@ -288,14 +288,14 @@ int product(const void* x, long long ldx, const void* w, long long ldw, const vo
     if (((uintptr_t)x | (uintptr_t)w) % 16) LLME_REFUSE("gemm_int4: operands must be 16-byte aligned");
     if (ldo < N) LLME_REFUSE("gemm_int4: output row stride shorter than the row");
     const long long groups = (K + group - 1LL) / group;
-    if (meets(span(out, M, N, ldo, out_f32 ? 4 : 2), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
+    if (meets(span(out, M, N, ldo, sizeof(O)), {span(x, M, K, ldx, 2), span(w, N, (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES, ldw, 1), span(scales, N, groups, lds, 2), span(zeros, N, groups, lds, 1)}))
         LLME_REFUSE("gemm_int4: the output lies over an operand");
-    Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, out, out_f32, ldo, M, N, K, 0};
+    Args a{(const bf16*)x, ldx, (const unsigned char*)w, ldw, (const bf16*)scales, (const unsigned char*)zeros, lds, out, ldo, M, N, K, 0};
     auto aligned = [&](int count) { return lds % count == 0 && (uintptr_t)scales % (2 * count) == 0 && (uintptr_t)zeros % count == 0; };
     a.together = aligned(256 / group) ? 2 : (aligned(128 / group) ? 1 : 0);
-    if (group == 32) return launch<1>(a, stream);
-    if (group == 64) return launch<2>(a, stream);
-    return launch<4>(a, stream);
+    if (group == 32) return launch<1, O>(a, stream);
+    if (group == 64) return launch<2, O>(a, stream);
+    return launch<4, O>(a, stream);
 }
 
 }  // namespace
@@ -305,12 +305,12 @@ int product(const void* x, long long ldx, const void* w, long long ldw, const vo
 // bfloat16, row stride ldo.
 LLME_API int llme_gemm_int4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds,
                             int group, void* out, long long ldo, int M, int N, int K, cudaStream_t stream) {
-    return product(x, ldx, w, ldw, scales, zeros, lds, group, out, 0, ldo, M, N, K, stream);
+    return product<bf16>(x, ldx, w, ldw, scales, zeros, lds, group, out, ldo, M, N, K, stream);
 }
 // The same with a 32-bit out: a sum on its way into the residual stream.
 LLME_API int llme_gemm_int4_f32(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, long long lds,
                                 int group, void* out, long long ldo, int M, int N, int K, cudaStream_t stream) {
-    return product(x, ldx, w, ldw, scales, zeros, lds, group, out, 1, ldo, M, N, K, stream);
+    return product<float>(x, ldx, w, ldw, scales, zeros, lds, group, out, ldo, M, N, K, stream);
 }
 
 // More than 16 tokens: 0 (the default): whichever kernel should be faster; 1: single SMs, K cut over clusters; 2: pairs of SMs.  For tests and

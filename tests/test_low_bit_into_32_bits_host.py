@@ -1,12 +1,10 @@
-"""What a sublayer of 4-bit weights adds to the residual stream is 32-bit, as with every other kind of weights; the entry point that writes it."""
+"""What a sublayer of 4-bit weights adds to the residual stream is 32-bit, as with every other kind of weights."""
 import pytest
 import torch
 
 from helpers import engine_for, make_model_dir, random_ids
 from low_bit_cases import LowBitOps, PlainLowBit
 from llmengine_b200.engine.engine import StepEntry
-from test_launchers_host import compiled  # noqa: F401  (the fixture)
-from test_low_bit_launchers_host import INT4, INT4_TYPES, call, p, refused
 from tiny_configs import TINY_A, TINY_B, TINY_C
 
 
@@ -46,23 +44,3 @@ def test_the_stream_holds_32_bits(tmp_path, cfg, form):
     rounded, kept = PlainLowBit(folder, "int4", *more).logits(ids), Plain32(folder, "int4", *more).logits(ids)
     # a stream whose additions are rounded to bfloat16 is farther from the engine's than one whose additions are not
     assert (got - kept).norm() < 0.5 * (got - rounded).norm()
-
-
-def test_the_entry_point(compiled):  # noqa: F811
-    lib = compiled("gemm_int4")
-    cases = [dict(K=60), dict(K=0), dict(ldx=68), dict(ldx=56), dict(ldw=48), dict(ldw=72), dict(lds=1), dict(group=16), dict(group=0), dict(ldo=47), dict(x=p(1, 8)),
-             dict(w=p(2, 8)), dict(out=p(1)), dict(out=p(2, 64)), dict(out=p(3)), dict(out=p(4))]
-    refused(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, [{k: None} for k in ("x", "w", "scales", "out")] + cases)
-    # four bytes a value: an output that ends before the operand behind it in bfloat16 lies over it in 32 bits
-    near = dict(out=p(1, -300), M=3)
-    assert call(lib, "llme_gemm_int4", INT4_TYPES, INT4, **near)[0] == 0
-    assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, **near)[0] == -1
-    for changed in (dict(M=0), dict(N=0)):
-        assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, **changed) == (0, 0)
-    for device in (0, 1, 65):
-        lib.fake_device(device)
-        for m in (1, 16, 17, 77, 300, 4096):
-            for group in (32, 64, 128):
-                assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, M=m, N=4096, K=4096, ldx=4096, ldw=2048, lds=4096 // group, group=group, ldo=4096, w=p(64),
-                            scales=p(90), zeros=p(100) if group == 32 else None, out=p(128)) == (0, 1)
-    lib.fake_device(0)

@@ -118,3 +118,23 @@ def test_every_size_is_launched_on_every_device(compiled):  # noqa: F811
                         assert call(int4, "llme_gemm_int4", INT4_TYPES, INT4, M=m, N=n, K=k, ldx=k, ldw=k // 2, lds=k // group, group=group, ldo=n, w=p(64), scales=p(90),
                                     zeros=p(100) if group == 32 else None, out=p(128)) == (0, 1)
     e4m3.fake_device(0), int4.fake_device(0)
+
+
+def test_products_of_4_bits_into_32_bits(compiled):  # noqa: F811
+    lib = compiled("gemm_int4")
+    cases = [dict(K=60), dict(K=0), dict(ldx=68), dict(ldx=56), dict(ldw=48), dict(ldw=72), dict(lds=1), dict(group=16), dict(group=0), dict(ldo=47), dict(x=p(1, 8)),
+             dict(w=p(2, 8)), dict(out=p(1)), dict(out=p(2, 64)), dict(out=p(3)), dict(out=p(4))]
+    refused(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, [{k: None} for k in ("x", "w", "scales", "out")] + cases)
+    # four bytes a value: an output that ends before the operand behind it in bfloat16 lies over it in 32 bits
+    near = dict(out=p(1, -300), M=3)
+    assert call(lib, "llme_gemm_int4", INT4_TYPES, INT4, **near)[0] == 0
+    assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, **near)[0] == -1
+    for changed in (dict(M=0), dict(N=0)):
+        assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, **changed) == (0, 0)
+    for device in (0, 1, 65):
+        lib.fake_device(device)
+        for m in (1, 16, 17, 77, 300, 4096):
+            for group in (32, 64, 128):
+                assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, M=m, N=4096, K=4096, ldx=4096, ldw=2048, lds=4096 // group, group=group, ldo=4096, w=p(64),
+                            scales=p(90), zeros=p(100) if group == 32 else None, out=p(128)) == (0, 1)
+    lib.fake_device(0)
