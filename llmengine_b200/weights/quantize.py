@@ -67,7 +67,7 @@ def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> Tup
     g = torch.nn.functional.pad(w, (0, -k % group)).view(n, -1, group)
     if zeros:
         least, most = g.amin(2).clamp(max=0.0), g.amax(2).clamp(min=0.0)
-        scales = ((most - least) / 15).clamp(min=LEAST).to(torch.bfloat16)
+        scales = ((most / 2 - least / 2) / 7.5).clamp(min=LEAST).to(torch.bfloat16)        # (halves: a span may be twice the largest number)
         at = (-least / scales.float()).round().clamp(0, 15)
     else:
         scales = (g.abs().amax(2) / 7).clamp(min=LEAST).to(torch.bfloat16)

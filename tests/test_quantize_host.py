@@ -67,3 +67,24 @@ def test_refusals():
                  lambda: qz.pack_int4(torch.zeros(2, 64)), lambda: qz.unpack_int4(torch.zeros(2, 64, dtype=torch.uint8), 129)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_the_largest_numbers_in_4_bits(zeros):
+    """A group whose largest and least values are farther apart than the largest 32-bit number."""
+    w = torch.zeros(3, 64)
+    w[0, 0], w[0, 1], w[1, 40] = 3e38, -3e38, -2.5e38
+    packed, scales, zero = qz.quantize_int4(w, 32, zeros)
+    back = qz.dequantize_int4(packed, scales, zero, 64, 32)
+    # half a step, the scale's rounding over the whole span, and with a zero point its half step (test_4_bits_are_near)
+    step = scales.float().repeat_interleave(32, 1)
+    assert torch.isfinite(scales.float()).all() and torch.all((back / step - w / step).abs() <= 0.5 + (0.5 if zeros else 0.0) + 15 * 2.0 ** -8)
+
+
+def test_spans_that_fit_are_rounded_as_they_were():
+    w = torch.cat([_w(64, 256, seed=s) * scale for s, scale in ((1, 1.0), (2, 1e-6), (3, 1e30))])
+    packed, scales, zero = qz.quantize_int4(w, 64, True)
+    g = w.view(len(w), -1, 64)
+    least, most = g.amin(2).clamp(max=0.0), g.amax(2).clamp(min=0.0)
+    assert torch.equal(scales, ((most - least) / 15).to(torch.bfloat16))
+    assert torch.equal(zero, (-least / scales.float()).round().clamp(0, 15).to(torch.uint8))
