@@ -42,9 +42,9 @@ def pack_int4(codes: torch.Tensor) -> torch.Tensor:
     if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
         raise ValueError("a code is outside 0..15")
     n, k = codes.shape
-    v = torch.nn.functional.pad(codes.to(torch.uint8), (0, -k % BLOCK)).view(n, -1, 4, 4, 2, 2, 2)     # block, j, q, byte, nibble, odd
+    v = torch.nn.functional.pad(codes.to(torch.uint8), (0, -k % BLOCK)).view(n, -(-k // BLOCK), 4, 4, 2, 2, 2)     # block, j, q, byte, nibble, odd
     v = v.permute(0, 1, 3, 2, 6, 4, 5)                                                                # block, q, j, odd, byte, nibble
-    return (v[..., 0] | (v[..., 1] << 4)).reshape(n, -1).contiguous()
+    return (v[..., 0] | (v[..., 1] << 4)).reshape(n, -(-k // BLOCK) * (BLOCK // 2)).contiguous()
 
 
 def unpack_int4(packed: torch.Tensor, k: int) -> torch.Tensor:
@@ -52,8 +52,8 @@ def unpack_int4(packed: torch.Tensor, k: int) -> torch.Tensor:
     n = packed.shape[0]
     if packed.dtype != torch.uint8 or packed.shape[1] != -(-k // BLOCK) * (BLOCK // 2):
         raise ValueError(f"{k} codes a row take uint8 rows of {-(-k // BLOCK) * (BLOCK // 2)}, got {packed.dtype} {tuple(packed.shape)}")
-    v = torch.stack([packed & 15, packed >> 4], -1).view(n, -1, 4, 4, 2, 2, 2)                        # block, q, j, odd, byte, nibble
-    return v.permute(0, 1, 3, 2, 5, 6, 4).reshape(n, -1)[:, :k].contiguous()
+    v = torch.stack([packed & 15, packed >> 4], -1).view(n, -(-k // BLOCK), 4, 4, 2, 2, 2)                        # block, q, j, odd, byte, nibble
+    return v.permute(0, 1, 3, 2, 5, 6, 4).reshape(n, -(-k // BLOCK) * BLOCK)[:, :k].contiguous()
 
 
 def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
@@ -64,7 +64,7 @@ def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> Tup
         raise ValueError(f"a group is of {', '.join(map(str, GROUPS))} values, got {group}")
     w = _finite(w)
     n, k = w.shape
-    g = torch.nn.functional.pad(w, (0, -k % group)).view(n, -1, group)
+    g = torch.nn.functional.pad(w, (0, -k % group)).view(n, -(-k // group), group)
     if zeros:
         least, most = g.amin(2).clamp(max=0.0), g.amax(2).clamp(min=0.0)
         scales = ((most / 2 - least / 2) / 7.5).clamp(min=LEAST).to(torch.bfloat16)        # (halves: a span may be twice the largest number)
@@ -73,7 +73,7 @@ def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> Tup
         scales = (g.abs().amax(2) / 7).clamp(min=LEAST).to(torch.bfloat16)
         at = torch.full_like(scales, 8.0, dtype=torch.float32)
     codes = (g / scales.float()[..., None] + at[..., None]).round().clamp(0, 15)
-    return pack_int4(codes.view(n, -1)[:, :k].to(torch.uint8)), scales, at.to(torch.uint8) if zeros else None
+    return pack_int4(codes.flatten(1)[:, :k].to(torch.uint8)), scales, at.to(torch.uint8) if zeros else None
 
 
 def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], k: int, group: int) -> torch.Tensor:

@@ -88,3 +88,15 @@ def test_spans_that_fit_are_rounded_as_they_were():
     least, most = g.amin(2).clamp(max=0.0), g.amax(2).clamp(min=0.0)
     assert torch.equal(scales, ((most - least) / 15).to(torch.bfloat16))
     assert torch.equal(zero, (-least / scales.float()).round().clamp(0, 15).to(torch.uint8))
+
+
+@pytest.mark.parametrize("n,k", [(0, 64), (0, 200), (3, 0)])
+def test_matrices_without_values(n, k):
+    packed = qz.pack_int4(torch.zeros(n, k, dtype=torch.uint8))
+    assert packed.shape == (n, -(-k // 128) * 64) and qz.unpack_int4(packed, k).shape == (n, k)
+    for zeros in (False, True):
+        packed, scales, zero = qz.quantize_int4(torch.zeros(n, k), 64, zeros)
+        assert scales.shape == (n, -(-k // 64)) and (zero is None or zero.shape == scales.shape)
+        assert qz.dequantize_int4(packed, scales, zero, k, 64).shape == (n, k)
+    q, scales = qz.quantize_e4m3(torch.zeros(n, k))
+    assert q.shape == (n, k) and scales.shape == (n,)
