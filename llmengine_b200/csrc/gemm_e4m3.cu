@@ -171,6 +171,7 @@ LLME_API int llme_gemm_e4m3(const void* x, long long ldx, const float* xs, const
                             int out_dtype, long long ldo, int M, int N, int K, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !xs || !w || !ws || !out) LLME_REFUSE("gemm_e4m3: null pointer");
+    if (M > MOST || N > MOST || K > MOST) LLME_REFUSE("gemm_e4m3: %d x %d x %d, at most %d of each", M, N, K, MOST);
     if (K <= 0 || K % 16 || ldx % 16 || ldw % 16 || ldx < K || ldw < K) LLME_REFUSE("gemm_e4m3: K=%d ldx=%lld ldw=%lld is not supported (multiples of 16, rows that do not overlap)", K, ldx, ldw);
     if (((uintptr_t)x | (uintptr_t)w) % 16) LLME_REFUSE("gemm_e4m3: operands must be 16-byte aligned");
     if (ldo < N) LLME_REFUSE("gemm_e4m3: output row stride shorter than the row");

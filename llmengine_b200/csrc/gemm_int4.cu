@@ -281,6 +281,7 @@ int product(const void* x, long long ldx, const void* w, long long ldw, const vo
             int M, int N, int K, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !w || !scales || !out) LLME_REFUSE("gemm_int4: null pointer");
+    if (M > MOST || N > MOST || K > MOST) LLME_REFUSE("gemm_int4: %d x %d x %d, at most %d of each", M, N, K, MOST);
     if (K <= 0 || K % 8 || ldx % 8 || ldx < K) LLME_REFUSE("gemm_int4: K=%d ldx=%lld is not supported (multiples of 8, rows that do not overlap)", K, ldx);
     if (group != 32 && group != 64 && group != 128) LLME_REFUSE("gemm_int4: groups of %d values are not supported (32, 64 or 128)", group);
     if (ldw % 16 || ldw < (K + BLOCK_K - 1LL) / BLOCK_K * BLOCK_BYTES) LLME_REFUSE("gemm_int4: rows of %lld bytes do not hold %d values in whole blocks", ldw, K);

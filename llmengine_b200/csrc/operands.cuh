@@ -1,8 +1,12 @@
-// Where an entry point's operands lie, so that it can refuse outputs that lie over what is read.
+// How large an entry point's operands may be and where they lie, so that it can refuse outputs that lie over what is read.
 #pragma once
 
 #include <initializer_list>
 #include <stdint.h>
+
+// The most rows, and values of one, that an entry point takes: its kernels count both in 32 bits and go past the last one, by a block's tiles or the
+// pieces of its warps at most, before they ask.
+constexpr int MOST = 0x7fffffff - 8192;
 
 struct Span { uintptr_t first, end, width, pitch; };       // bytes: from, to, of a row, from row to row; empty where there is no operand
 

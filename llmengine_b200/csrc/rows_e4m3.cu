@@ -381,6 +381,7 @@ LLME_API int llme_rmsnorm_e4m3(const float* x, const void* delta, int delta_dtyp
                                void* q, float* scales, int rows, int size, float eps, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (!x || !gain || !q || !scales || size <= 0) LLME_REFUSE("rmsnorm_e4m3: null pointer or non-positive size");
+    if (rows > MOST || size > MOST) LLME_REFUSE("rmsnorm_e4m3: %d rows of %d values, at most %d of either", rows, size, MOST);
     if (delta && !total) LLME_REFUSE("rmsnorm_e4m3: a contribution needs a place for the sum");
     if (!(eps > 0.0f)) LLME_REFUSE("rmsnorm_e4m3: eps must be positive");
     const Span at_x = span(x, rows, size, size, 4), at_delta = span(delta, rows, size, size, bytes_of(delta_dtype)), at_gain = span(gain, 1, size, size, bytes_of(gain_dtype));
@@ -400,6 +401,7 @@ LLME_API int llme_rmsnorm_e4m3(const float* x, const void* delta, int delta_dtyp
 LLME_API int llme_rows_e4m3(const void* x, int dtype, long long ldx, void* q, long long ldq, float* scales, int rows, int size, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (!x || !q || !scales || size <= 0) LLME_REFUSE("rows_e4m3: null pointer or non-positive size");
+    if (rows > MOST || size > MOST) LLME_REFUSE("rows_e4m3: %d rows of %d values, at most %d of either", rows, size, MOST);
     if (ldx < size || ldq < size) LLME_REFUSE("rows_e4m3: a row stride is shorter than the row");
     const Span at_x = span(x, rows, size, ldx, bytes_of(dtype)), at_q = span(q, rows, size, ldq, 1), at_scales = span(scales, 1, rows, rows, 4);
     if (meets(at_q, {at_x, at_scales}) || meets(at_scales, {at_x})) LLME_REFUSE("rows_e4m3: an output lies over another operand");
@@ -413,6 +415,7 @@ LLME_API int llme_rows_e4m3(const void* x, int dtype, long long ldx, void* q, lo
 LLME_API int llme_swiglu_e4m3(const void* x, int dtype, long long ldx, void* q, long long ldq, float* scales, int rows, int size, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (!x || !q || !scales || size <= 0) LLME_REFUSE("swiglu_e4m3: null pointer or non-positive size");
+    if (rows > MOST || size > MOST) LLME_REFUSE("swiglu_e4m3: %d rows of %d values, at most %d of either", rows, size, MOST);
     if (ldx < 2LL * size || ldq < size) LLME_REFUSE("swiglu_e4m3: a row stride is shorter than the row");
     const Span at_x = span(x, rows, 2LL * size, ldx, bytes_of(dtype)), at_q = span(q, rows, size, ldq, 1), at_scales = span(scales, 1, rows, rows, 4);
     if (meets(at_q, {at_x, at_scales}) || meets(at_scales, {at_x})) LLME_REFUSE("swiglu_e4m3: an output lies over another operand");

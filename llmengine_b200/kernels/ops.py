@@ -37,6 +37,7 @@ class KernelError(RuntimeError):
 _F32, _BF16 = 0, 1
 _F32T, _BF16T, _F8, _BYTE = torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8
 _FLOAT, _FLOATS, _BF16S, _E4M3, _BYTES = (_F32T,), (_F32T, _BF16T), (_BF16T,), (_F8,), (_BYTE,)
+_MOST = (1 << 31) - 1 - 8192            # rows, and values of one, that these methods take: their kernels' indices are 32-bit (csrc/operands.cuh)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
@@ -395,6 +396,8 @@ class CudaOps:
             raise KernelError(f"{what}: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
         if t.shape != shape if shape is not None else t.dim() != 2:
             raise KernelError(f"{what}: {name} must {'be a matrix' if shape is None else f'have shape {tuple(shape)}'}, got shape {tuple(t.shape)}")
+        if max(t.shape) > _MOST:
+            raise KernelError(f"{what}: {name} may have at most {_MOST} rows and values a row, got shape {tuple(t.shape)}")
         if not t.is_contiguous() and (dense or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1)):
             raise KernelError(f"{what}: {name} must {'be contiguous' if dense else 'have rows without gaps'}, got strides {tuple(t.stride())}")
         return t
@@ -604,7 +607,7 @@ class CudaOps:
                 and x.dim() == 2 and x.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
             rows, cols = x.shape
             size = cols // halves
-            if out.shape == (rows, size) and scales.shape == (rows,) and cols and size * halves == cols:
+            if out.shape == (rows, size) and scales.shape == (rows,) and cols and size * halves == cols and rows <= _MOST and cols <= _MOST:
                 return rows, size, cols, size
         rows, cols = self._operand(what, name, x, _FLOATS).shape
         if cols % halves:
@@ -677,7 +680,7 @@ class CudaOps:
         M, K = self._operand(what, "x", x, _E4M3).shape
         if not (x_scales.get_device() == d == w.get_device() and w_scales.get_device() == d == out.get_device() and w.dtype is _F8
                 and x_scales.dtype is _F32T and w_scales.dtype is _F32T and out.dtype in _FLOATS and w.dim() == 2 and w.shape[1] == K
-                and x_scales.shape == (M,) and w_scales.shape == w.shape[:1] and out.shape == (M, w.shape[0])
+                and x_scales.shape == (M,) and w_scales.shape == w.shape[:1] and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST
                 and x_scales.is_contiguous() and w_scales.is_contiguous() and out.is_contiguous() and w.is_contiguous()):
             N, width = self._operand(what, "w", w, _E4M3).shape
             if width != K:
@@ -719,7 +722,7 @@ class CudaOps:
         M, K = self._operand(what, "x", x, _BF16S).shape
         if not (w.get_device() == d == scales.get_device() and out.get_device() == d and w.dtype is _BYTE and scales.dtype is _BF16T
                 and out.dtype is _BF16T and w.dim() == 2 == scales.dim() and w.shape[0] == scales.shape[0] and w.shape[1] == (K + 127) // 128 * 64
-                and out.shape == (M, w.shape[0]) and w.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
+                and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST and w.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
             N, width = self._operand(what, "w", w, _BYTES).shape
             if width != (K + 127) // 128 * 64:
                 raise KernelError(f"{what}: {K} codes a row take {(K + 127) // 128 * 64} bytes, w has {width}")

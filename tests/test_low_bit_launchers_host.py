@@ -138,3 +138,33 @@ def test_products_of_4_bits_into_32_bits(compiled):  # noqa: F811
                 assert call(lib, "llme_gemm_int4_f32", INT4_TYPES, INT4, M=m, N=4096, K=4096, ldx=4096, ldw=2048, lds=4096 // group, group=group, ldo=4096, w=p(64),
                             scales=p(90), zeros=p(100) if group == 32 else None, out=p(128)) == (0, 1)
     lib.fake_device(0)
+
+
+def test_sizes_at_the_end_of_32_bits(compiled):  # noqa: F811
+    """Indices go a block's width past the last value: sizes that leave no room for that below 2^31 are refused, the largest that do are launched."""
+    rows, e4m3, int4 = compiled("rows_e4m3"), compiled("gemm_e4m3"), compiled("gemm_int4")
+    far = dict(x=p(1), q=p(1 << 12), scales=p(1 << 13))
+    most = 0x7FFFFFFF - 8192
+    for entry, more in (("llme_rows_e4m3", 1), ("llme_swiglu_e4m3", 2)):
+        for size, n in ((most, 1), (2, most)):
+            given = {**ROWS, **far, "rows": n, "size": size, "ldx": more * size, "ldq": size}
+            assert call(rows, entry, ROWS_TYPES, given) == (0, 1)
+            for changed in (dict(rows=n + 1) if n == most else dict(size=size + 1, ldx=more * (size + 1), ldq=size + 1), dict(rows=0x7FFFFFFF), dict(size=0x7FFFFFFF, ldx=1 << 40, ldq=1 << 40)):
+                assert call(rows, entry, ROWS_TYPES, given, **changed) == (-1, 0)
+    wide = dict(x=p(1), delta=p(1 << 20), total=p(1), q=p(2 << 20), scales=p(3 << 20), gain=p(4 << 20))
+    for changed in (dict(size=most), dict(rows=most)):
+        assert call(rows, "llme_rmsnorm_e4m3", NORM_TYPES, {**NORM, **wide}, **changed) == (0, 1)
+        changed = {k: v + 1 for k, v in changed.items()}
+        assert call(rows, "llme_rmsnorm_e4m3", NORM_TYPES, {**NORM, **wide}, **changed) == (-1, 0)
+    spread = dict(x=p(1), w=p(1 << 14), out=p(1 << 16))
+    large = most // 128 * 128
+    for lib, entry, types, given in ((e4m3, "llme_gemm_e4m3", E4M3_TYPES, {**E4M3, **spread, "xs": p(1 << 18), "ws": p(1 << 19)}),
+                                     (int4, "llme_gemm_int4", INT4_TYPES, {**INT4, **spread, "scales": p(1 << 18), "zeros": p(1 << 19)}),
+                                     (int4, "llme_gemm_int4_f32", INT4_TYPES, {**INT4, **spread, "scales": p(1 << 18), "zeros": p(1 << 19)})):
+        for changed in (dict(M=most), dict(N=most, ldo=most)):
+            assert call(lib, entry, types, given, **changed) == (0, 1), (entry, changed)
+            assert call(lib, entry, types, given, **{k: v + 1 for k, v in changed.items()}) == (-1, 0)
+        deep = dict(K=large, ldx=large, ldw=large, **(dict(lds=large // 32) if "int4" in entry else {}))
+        for m in (1, 40):
+            assert call(lib, entry, types, given, M=m, **deep) == (0, 1)
+            assert call(lib, entry, types, given, M=m, **{**deep, "K": large + 128, "ldx": 1 << 40, "ldw": 1 << 40, **(dict(lds=1 << 40) if "int4" in entry else {})}) == (-1, 0)
