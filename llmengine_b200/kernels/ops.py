@@ -603,12 +603,15 @@ class CudaOps:
     def _rows_of(self, what: str, name: str, x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, halves: int):
         """(rows, values of an output row, row stride of x, row stride of out) for 8-bit rows of x, `halves` of its columns an output value."""
         d = self._device_index
-        if (x.get_device() == d == out.get_device() and scales.get_device() == d and x.dtype in _FLOATS and out.dtype is _F8 and scales.dtype is _F32T
-                and x.dim() == 2 and x.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
-            rows, cols = x.shape
-            size = cols // halves
-            if out.shape == (rows, size) and scales.shape == (rows,) and cols and size * halves == cols and rows <= _MOST and cols <= _MOST:
-                return rows, size, cols, size
+        try:
+            if (x.get_device() == d == out.get_device() and scales.get_device() == d and x.dtype in _FLOATS and out.dtype is _F8 and scales.dtype is _F32T
+                    and x.dim() == 2 and x.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
+                rows, cols = x.shape
+                size = cols // halves
+                if out.shape == (rows, size) and scales.shape == (rows,) and cols and size * halves == cols and rows <= _MOST and cols <= _MOST:
+                    return rows, size, cols, size
+        except AttributeError:               # (no tensor: said below)
+            pass
         rows, cols = self._operand(what, name, x, _FLOATS).shape
         if cols % halves:
             raise KernelError(f"{what}: {name} must have an even number of columns, got {cols}")
@@ -630,9 +633,13 @@ class CudaOps:
         what = "rmsnorm_e4m3"
         rows, size = self._operand(what, "x", x, _FLOAT, dense=True).shape
         d, shape = self._device_index, x.shape
-        if not (gain.get_device() == d == out.get_device() and scales.get_device() == d and gain.dtype in _FLOATS and out.dtype is _F8
-                and scales.dtype is _F32T and gain.shape == (size,) and out.shape == shape and scales.shape == (rows,) and size
-                and gain.is_contiguous() and out.is_contiguous() and scales.is_contiguous()):
+        try:
+            usual = (gain.get_device() == d == out.get_device() and scales.get_device() == d and gain.dtype in _FLOATS and out.dtype is _F8
+                     and scales.dtype is _F32T and gain.shape == (size,) and out.shape == shape and scales.shape == (rows,) and size
+                     and gain.is_contiguous() and out.is_contiguous() and scales.is_contiguous())
+        except AttributeError:
+            usual = False
+        if not usual:
             self._operand(what, "gain", gain, _FLOATS, (size,), dense=True)
             self._places8(what, rows, size, out, scales, dense=True)
         if not eps > 0.0:
@@ -678,10 +685,14 @@ class CudaOps:
         or bfloat16; sums are 32-bit.  K is a multiple of 16, the rows of x and w begin on 16 bytes (any such row stride)."""
         what, d = "linear_e4m3", self._device_index
         M, K = self._operand(what, "x", x, _E4M3).shape
-        if not (x_scales.get_device() == d == w.get_device() and w_scales.get_device() == d == out.get_device() and w.dtype is _F8
-                and x_scales.dtype is _F32T and w_scales.dtype is _F32T and out.dtype in _FLOATS and w.dim() == 2 and w.shape[1] == K
-                and x_scales.shape == (M,) and w_scales.shape == w.shape[:1] and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST
-                and x_scales.is_contiguous() and w_scales.is_contiguous() and out.is_contiguous() and w.is_contiguous()):
+        try:
+            usual = (x_scales.get_device() == d == w.get_device() and w_scales.get_device() == d == out.get_device() and w.dtype is _F8
+                     and x_scales.dtype is _F32T and w_scales.dtype is _F32T and out.dtype in _FLOATS and w.dim() == 2 and w.shape[1] == K
+                     and x_scales.shape == (M,) and w_scales.shape == w.shape[:1] and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST
+                     and x_scales.is_contiguous() and w_scales.is_contiguous() and out.is_contiguous() and w.is_contiguous())
+        except AttributeError:
+            usual = False
+        if not usual:
             N, width = self._operand(what, "w", w, _E4M3).shape
             if width != K:
                 raise KernelError(f"{what}: rows of {K} values and weight rows of {width}")
@@ -720,9 +731,13 @@ class CudaOps:
         of 8, the rows of x and w begin on 16 bytes (any such row stride).  (Into 32 bits: the plan's record, `Plan.linear_int4`.)"""
         what, d = "linear_int4", self._device_index
         M, K = self._operand(what, "x", x, _BF16S).shape
-        if not (w.get_device() == d == scales.get_device() and out.get_device() == d and w.dtype is _BYTE and scales.dtype is _BF16T
-                and out.dtype is _BF16T and w.dim() == 2 == scales.dim() and w.shape[0] == scales.shape[0] and w.shape[1] == (K + 127) // 128 * 64
-                and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST and w.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
+        try:
+            usual = (w.get_device() == d == scales.get_device() and out.get_device() == d and w.dtype is _BYTE and scales.dtype is _BF16T
+                     and out.dtype is _BF16T and w.dim() == 2 == scales.dim() and w.shape[0] == scales.shape[0] and w.shape[1] == (K + 127) // 128 * 64
+                     and out.shape == (M, w.shape[0]) and w.shape[0] <= _MOST and w.is_contiguous() and scales.is_contiguous() and out.is_contiguous())
+        except AttributeError:
+            usual = False
+        if not usual:
             N, width = self._operand(what, "w", w, _BYTES).shape
             if width != (K + 127) // 128 * 64:
                 raise KernelError(f"{what}: {K} codes a row take {(K + 127) // 128 * 64} bytes, w has {width}")

@@ -23,6 +23,15 @@ def _given():
             "linear_e4m3": (q, s, w8, ws, out), "linear_int4": (x.to(BF16), w4, sc, out.to(BF16))}
 
 
+@pytest.mark.parametrize("wrong", [None, 3.0, [1.0, 2.0]])
+def test_operands_that_are_no_tensors(ops, wrong):
+    for name, args in _given().items():
+        for i, a in enumerate(args):
+            if isinstance(a, torch.Tensor):
+                with pytest.raises(KernelError, match=name):
+                    getattr(ops, name)(*args[:i], wrong, *args[i + 1:])
+
+
 @pytest.mark.parametrize("many", [(1 << 31) - 8191, (1 << 31) + 64, (1 << 32) + 64])
 def test_more_rows_or_values_than_an_index_holds(ops, many):
     """(A size is handed on as a 32-bit number: one above 2^32 would look like a small one.)"""
