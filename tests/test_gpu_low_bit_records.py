@@ -34,3 +34,15 @@ def test_records(tmp_path, cfg, form):
         step(**tokens)
     eng.check_kernels()
     assert len(seen) == steps * len(eng.model.order) * (8 if form["weights"] == "e4m3" else 5)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=["e4m3", "int4", "int4-groups-of-32"])
+def test_records_beside_plain_kernels(tmp_path, form):
+    """The other operations by their plain kernels: what the records of low-bit weights are, does not follow from that choice."""
+    folder = make_model_dir(str(tmp_path), TINY_D, seed=3)
+    eng = engine_for(folder, "bfloat16", 256, kernels="plain", **form)
+    seen, ids = watch(eng), random_ids(60, TINY_D["vocab_size"], 5)
+    eng.step([StepEntry("a", ids[:50], [49])])
+    eng.step([StepEntry("a", ids[50:51], [0])])
+    eng.check_kernels()
+    assert len(seen) == 2 * len(eng.model.order) * (8 if form["weights"] == "e4m3" else 5)
