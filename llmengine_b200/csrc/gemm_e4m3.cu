@@ -6,7 +6,7 @@
 // each, for W and x alike, so that a lane's operands for two steps are 16 bytes of a row of W (two rows a lane), on their way through a ring
 // in shared memory (weight_stream.cuh), and one 16-byte load of a row of x.  8 x 6144 x 4096 6.8 us (3.7 TB/s), 8 x 24576 x 4096 19.5 (5.2 TB/s).
 // More: tcgen05, the weights on the lanes of tensor memory (gemm_wide.cuh: 77 x 4096 x 12288 14.6 us, 3.6 TB/s) or 256 x 256 tiles on pairs of
-// SMs (gemm_e4m3_pair.cuh: 2048 x 24576 x 4096 144 us, 2.86 PFLOP/s).
+// SMs (gemm_e4m3_pair.cuh: 2048 x 24576 x 4096 148 us, 2.8 PFLOP/s, at the 1.5 GHz that the power limit leaves; 178 after a second of it).
 //
 // The reference's products are cublasSgemm (src/runtime/kernels/cuda_kernels.cu:892-908); it has none of 8-bit floats.
 #include <cuda.h>
@@ -134,7 +134,7 @@ int launch_skinny(const Args& a, cudaStream_t s) {
 }
 
 // More tokens than the weight-streaming kernel takes at once: 256 x 256 tiles on pairs of SMs, or narrower tiles with K cut over a cluster,
-// whichever a model of its time says is faster.  A step of 128 values takes a pair 580 cycles, all tiles but the last 4,300 at least, which
+// whichever a model of its time says is faster (its cycles: wide::shape()).  A step of 128 values takes a pair 580 cycles, all tiles but the last 4,300 at least, which
 // the way out of the one before takes, and starting and the last one's way out some 9,800 (384 x 4096 x 512 / 4096: 5.4 / 14.2 us, 2048 x 24576 x
 // 128 29.2).
 template <typename O>

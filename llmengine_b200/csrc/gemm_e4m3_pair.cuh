@@ -7,8 +7,8 @@
 // accumulator is double-buffered.  Eight warps of each block read it back, multiply by the two scales and store through shared memory
 // (TMA; value by value where the output's rows do not begin on 16 bytes): 2048 x 24576 x 128, which is little else, 29 us in bfloat16 and
 // 37 in 32 bits (5.4 TB/s of output); rows of an odd length, 2048 x 10423 x 2576 in bfloat16, 58 us, straight from registers 256.  2048 x 24576 x
-// 4096 takes 138 to 147 us (2.8 to 3.0 PFLOP/s, the GPU's power decides which), the tensor pipe busy for 91 % of the time; behind other work, when the
-// clock has come down, 172.  The plumbing is that of the bfloat16 product on pairs
+// 4096 takes 138 to 148 us (2.8 to 3.0 PFLOP/s) at 1.5 GHz, to which the power limit brings the clock within one launch, the tensor pipe busy for
+// 91 % of the cycles in which its SM works and 82 % of all; after a second of it, at 1.15 GHz, 178.  The plumbing is that of the bfloat16 product on pairs
 // (gemm_tcgen05.cu); a step moves the same bytes and does twice the work.
 #pragma once
 

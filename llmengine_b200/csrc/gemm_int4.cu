@@ -10,8 +10,8 @@
 // Up to 16 tokens: bound by reading the codes.  As in the bfloat16 product (gemm_skinny.cu) 16 weight rows are the M side of a
 // mma.sync.m16n8k16 tile and the tokens its N side; the codes come through a ring in shared memory (weight_stream.cuh).  They enter the
 // instruction as (c - z) 2^-6; a group's sums are multiplied by its scale, in 32-bit, when the group ends: no weight is rounded.
-// 1 x 24576 x 4096, groups of 128: 14.1 us, 3.7 TB/s, where the loads alone take 10.1 and making numbers of the codes the rest; with zero points
-// 15.3, in groups of 32 with zero points 21.7.  1 x 17408 x 5120 12.9 us, 1 x 4096 x 4096 4.4.
+// 1 x 24576 x 4096, groups of 128: 13.6 us, 3.8 TB/s, where the loads alone take 10.1 and making numbers of the codes the rest; with zero points
+// 15.4, in groups of 32 with zero points 21.8 (x in L2; from memory 14.8, 17.4, 22.9).  1 x 17408 x 5120 13.0 us, 1 x 4096 x 4096 4.4.
 // More: tcgen05, the weights made into bfloat16 numbers in tensor memory, on single SMs (gemm_wide.cuh) or on pairs (gemm_int4_pair.cuh).
 //
 // The reference's weight-only product has 8-bit blocks (src/runtime/kernels/cuda_kernels.cu:296-358); it has none of 4 bits.

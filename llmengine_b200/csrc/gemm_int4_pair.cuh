@@ -12,7 +12,9 @@
 //     cycles from step to step, a third of them waits and messages: two sets were slower than the instructions, which take 768 at 192 tokens);
 //   * four warps read the block's half of the accumulator, which is double-buffered, and store it, a token's 32 neighbouring values at a time
 //     (1999 x 8192 x 256, little else: 17 us; through shared memory and TMA 25).
-// 1900 x 7168 x 5120 takes 92 us (1.51 PFLOP/s), the tensor pipe busy for 88 % of the time.
+// 1900 x 7168 x 5120 takes 92 to 94 us (1.5 PFLOP/s) at 1.53 GHz, to which the power limit brings the clock within one launch, the tensor pipe busy for
+// 88 % of the cycles in which its SM works and 77 % of all (280 tiles, 74 pairs); after a second of it, at 1.37 GHz, 114.  In groups of 32 with zero
+// points 108 and 130.
 // The accumulators take 2 NT columns of tensor memory and the weights the rest, 64 columns a step: NT is at most 192.
 // All waits are bounded (umma.cuh).
 #pragma once
@@ -299,7 +301,7 @@ int pairs_held() {
     return n;
 }
 
-// The tile width that takes the fewest cycles, and how many: a step takes 780 and one for every token of the tile (1900 x 7168 x 5120, tiles of 64 /
+// The tile width that takes the fewest cycles (as in wide::shape(): microseconds times 1,870), and how many: a step takes 780 and one for every token of the tile (1900 x 7168 x 5120, tiles of 64 /
 // 128 / 160 / 192: 226 / 124 / 113 / 92 us), the way from one tile to the next 1,500; all tiles but the last take 4,000 and three for every token at
 // least, which the way out of the one before takes (768 / 1600 x 24576 x 256: 17.8 / 32.7 us); starting takes 3,300, the last one's way out 23 for
 // every token.

@@ -387,10 +387,14 @@ int clusters_held(int segments, int per_sm) {
 // (as many as are held) share the memory's 4,000 bytes a cycle for the weights; an SM's blocks share its 60 bytes a cycle from L2 (52 beside the
 // making of numbers) and its tensor core, where a step takes twice nt cycles (128 e4m3 values) or four times (bfloat16); making numbers of a step's
 // codes keeps an SM busy for 850.  Starting and ending a block cost about 4,000 cycles and 22 for every token, the cluster's sums 3,000 and 10.
+// All of these models count microseconds times 1,870.  (The clock is 1,965 MHz until the power limit holds it: many tokens' products run at 1.5 GHz, and
+// what is 972 here, a step of 192 tokens on pairs in 4 bits, is some 780 of the SM's own cycles, its instructions' 768 and little else.)
 // Over 42 products of 40 to 1,600 tokens and all of their tilings the model is off by 12 % (standard deviation), and its choice took 1 % longer than
-// the best with 8 bits, 2 % with 4.  (200 x 4096 x 4096 in 8 bits, tiles of 208 tokens in four segments, 10.7 us; 96 x 7168 x 5120 in 4 bits, two
-// segments, 15.6, where tiles of 48, two blocks an SM, take 31.  Tiles a quarter as wide as the widest are for few weight rows: 2048 x 264 x 1616 in
-// 8 bits 7.0 us, with tiles of 192 to 256 alone 9.1.)
+// the best with 8 bits, 2 % with 4.  (200 x 4096 x 4096 in 8 bits, tiles of 208 tokens in four segments, 11.3 us; 96 x 7168 x 5120 in 4 bits, two
+// segments, 15.6, where tiles of 48, two blocks an SM, take 31.)
+// Widths: as few tiles along the tokens as a width of 256 allows, and one, two and three more, one by one; from there in steps of half of what has been
+// reached, up to four times the fewest and three, for few weight rows, whose wide tiles would leave SMs idle (2048 x 264 x 1616 in 8 bits 7.2 us, with
+// tiles of 192 to 256 alone 9.1).  Not every width: a call asks the model about each.
 template <bool INT4, int RUNS, bool ZEROS>
 int shape(Args& g, double* cycles) {
     const int steps = (g.K + STEP - 1) / STEP, n_tiles = (g.N + BM - 1) / BM, w_bytes = INT4 ? BM * STEP / 2 : BM * STEP, x_width = STEP * (INT4 ? 2 : 1);

@@ -11,10 +11,11 @@
 //     the squares and m, and the block meets once: a = max(r m, 2^-100) / 448, q = t (r / a) g;
 //   * a matrix's rows as they are;
 //   * silu(gate) * up of a [gate | up] product.
-// All arithmetic is 32-bit; the squares are added in a fixed order that depends on the row's width alone.
+// All arithmetic is 32-bit; the squares are added in a fixed order that depends on the row's width and on how the operands are aligned, not on the
+// other rows.
 //
 // Bound by memory: a row stays in registers between the two passes over it, so it is read once.  Norm of 1,999 x 5,120 with a bfloat16 delta
-// 18.7 us (6.0 TB/s), 4,096 x 4,096 bfloat16 rows 10.2 us (4.9 TB/s: in so short a time a launch's start and end weigh more), the gate of 2,048 x 17,408
+// 18.6 us (6.0 TB/s), 4,096 x 4,096 bfloat16 rows 10.2 us (4.9 TB/s: in so short a time a launch's start and end weigh more), the gate of 2,048 x 17,408
 // 31.4 us (5.7 TB/s); a handful of rows 1.2 to 2.5 us, a launch.
 // Reference counterpart: rmsnorm_kernel and fused_silu_mul (src/runtime/kernels/cuda_kernels.cu:360-378, :993-1002) write 32-bit rows;
 // the reference has no 8-bit rows.
