@@ -3,7 +3,7 @@
 // A warp owns 16 weight rows and walks over them in pieces of 128 bytes a row; lane (r, quad) = (lane / 4, lane % 4) needs of every piece the
 // 16 bytes at quad * 16 and at 64 + quad * 16 of rows r and r + 8.  The pieces of the next steps lie in a ring in shared memory, brought by
 // asynchronous copies: every lane copies what it will read itself, so nothing has to be shared and no barrier is met, and how much is under
-// way does not cost registers.  (24576 x 4096 in 4 bits, one token: 14.1 us, the loads alone 10.1; with the pieces in registers a warp's loads and
+// way does not cost registers.  (24576 x 4096 in 4 bits, one token: 13.6 us, the loads alone 10.1; with the pieces in registers a warp's loads and
 // its arithmetic took turns, 18.1 us.  A ring of three, four or six steps gains nothing.)
 // Where the row groups alone do not fill the GPU, several warps share a group: warp p of n takes the pieces p, p + n, ..., and their sums are
 // added in the order of the warps.  How many share follows from the weights' shape alone, so a token's result does not depend on the others.
